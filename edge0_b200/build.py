@@ -1,6 +1,7 @@
 """Builds edge0_b200/lib/libedge0_b200.so (the C-ABI library with the sm_100a kernels) with nvcc.
 
-Cross-compiles without a GPU.  Usage: python -m edge0_b200.build [--verbose]
+Cross-compiles without a GPU; the sources are compiled side by side, those whose headers have not changed are left as they are.
+Usage: python -m edge0_b200.build [--verbose] [--force]
 """
 from __future__ import annotations
 
@@ -10,9 +11,10 @@ import subprocess
 import sys
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
-SRC = [os.path.join(ROOT, "csrc", "capi.cu"), os.path.join(ROOT, "csrc", "gguf_reader.cpp")]
+SRC = sorted(os.path.join(ROOT, "csrc", f) for f in os.listdir(os.path.join(ROOT, "csrc")) if f.endswith((".cu", ".cpp")))
 DEPS = [os.path.join(ROOT, "csrc", f) for f in os.listdir(os.path.join(ROOT, "csrc"))] + [
     os.path.join(os.path.dirname(ROOT), "include", "edge0_b200_moe.h")]
+OBJ = os.path.join(ROOT, "lib", "build")
 LIB = os.path.join(ROOT, "lib", "libedge0_b200.so")
 
 
@@ -27,16 +29,46 @@ def up_to_date() -> bool:
     return os.path.exists(LIB) and all(os.path.getmtime(LIB) >= os.path.getmtime(d) for d in DEPS)
 
 
+def _object(src: str) -> str:
+    return os.path.join(OBJ, os.path.basename(src) + ".o")
+
+
+def _stale(src: str, flags: str) -> bool:
+    """Whether src has to be compiled: no object, other flags, or a file that it read (as the compiler wrote down) is newer."""
+    obj = _object(src)
+    try:
+        with open(obj + ".flags") as f:
+            if f.read() != flags:
+                return True
+        with open(obj + ".d") as f:
+            read = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+        return any(os.path.getmtime(d) > os.path.getmtime(obj) for d in read)
+    except (OSError, IndexError):
+        return True
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
-    os.makedirs(os.path.dirname(LIB), exist_ok=True)
-    cmd = [nvcc(), "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
-           "--shared", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-o", LIB] + SRC
+    os.makedirs(OBJ, exist_ok=True)
+    flags = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden"]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    cmd[1:1] = os.environ.get("B200MOE_NVCC_FLAGS", "").split()   # development switches, e.g. -DB200MOE_FP4_PROF
-    subprocess.check_call(cmd)
+        flags.insert(0, "-Xptxas=-v")
+    flags[:0] = os.environ.get("B200MOE_NVCC_FLAGS", "").split()   # development switches, e.g. -DB200MOE_FP4_PROF
+    running = []
+    for src in SRC:
+        if force or _stale(src, " ".join(flags)):
+            obj = _object(src)
+            if os.path.exists(obj + ".flags"):
+                os.remove(obj + ".flags")
+            running.append((src, subprocess.Popen([nvcc(), *flags, "-MMD", "-MF", obj + ".d", "-c", "-o", obj, src])))
+    failed = [src for src, p in running if p.wait()]
+    if failed:
+        raise RuntimeError("nvcc failed on " + ", ".join(os.path.basename(s) for s in failed))
+    for src, _ in running:
+        with open(_object(src) + ".flags", "w") as f:
+            f.write(" ".join(flags))
+    subprocess.check_call([nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "--shared", "-Xcompiler", "-fPIC", "-o", LIB] + [_object(s) for s in SRC])
     return LIB
 
 

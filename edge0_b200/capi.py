@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(ROOT, "lib", "libedge0_b200.so")
 TYPE_F32, TYPE_Q3_K, TYPE_BF16, TYPE_NVFP4 = 0, 11, 30, 40
 OK = 0
 NOALLOC_MAX_LOGITS = 32768  # B200MOE_NOALLOC_MAX_LOGITS
+KV_BF16, KV_Q8, KV_Q4 = 0, 1, 2
 STATUS = {0: "OK", 1: "INVALID_ARG", 2: "UNSUPPORTED", 3: "ALLOC", 4: "CUDA", 5: "DEVICE_CHECK", 6: "NO_DEVICE"}
 
 
@@ -33,6 +34,22 @@ class Observe(C.Structure):
 class Tensor(C.Structure):
     """b200moe_tensor: data pointer, ne[4] elements, nb[4] byte strides (ggml's description of a tensor)."""
     _fields_ = [("data", C.c_void_p), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("n_rot", C.c_int32), ("n_axes", C.c_int32), ("sections", C.c_int32 * 4), ("interleaved", C.c_int32), ("adjacent", C.c_int32),
+                ("inverse", C.c_int32), ("reserved_", C.c_int32), ("base", C.c_double)]
+
+
+class KvCacheDesc(C.Structure):
+    """b200moe_kv_cache"""
+    _fields_ = [(n, C.c_int32) for n in ("type", "n_head_kv", "head_dim", "page_size")] + [("n_pages", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+class Attn(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seq", "max_new", "max_kv_len", "prefix_len", "pages_stride")] + [("scale", C.c_float)] + [
+        (n, C.c_void_p) for n in ("q_start", "kv_len", "pages", "prefix_pages")]
 
 
 class Counters(C.Structure):
@@ -94,6 +111,13 @@ SIGNATURES = {
     "b200moe_op_soft_max": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_float, C.c_void_p]),
     "b200moe_op_argsort_desc": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p]),
     "b200moe_op_mul_mat_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "b200moe_op_rope": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int, C.c_void_p, C.POINTER(Rope), C.POINTER(Tensor), C.c_void_p]),
+    "b200moe_kv_cache_bytes": (C.c_int, [C.POINTER(KvCacheDesc), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+    "b200moe_kv_write": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Tensor), C.POINTER(Tensor), C.c_int, C.c_void_p, C.c_void_p]),
+    "b200moe_kv_read": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_int, C.c_void_p]),
+    "b200moe_attention_workspace": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Attn), C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "b200moe_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Attn), C.POINTER(Tensor), C.c_int, C.POINTER(Tensor), C.c_void_p,
+                                    C.c_void_p, C.c_size_t, C.c_void_p]),
     "b200moe_probe_fp4_tile": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200moe_probe_fp4_rate": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]),
     "b200moe_route_noalloc": (C.c_int, [C.c_int, C.POINTER(Layer), C.c_void_p, C.c_int, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,

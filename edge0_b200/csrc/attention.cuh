@@ -1,0 +1,778 @@
+// Attention of a batch of sequences over the paged cache (kv_cache.cuh), behind a prefix that all of them may share.
+//
+// Token t of sequence b sees the prefix's positions and then its own 0 .. seen - 1, seen = kv_len[b] - new[b] + (place of t among the
+// sequence's new tokens) + 1.  For each of its heads: s_j = scale * q . k_j, out = sum_j softmax(s)_j v_j.
+//
+// The query heads that read one key/value head, of all tokens of a sequence (for the prefix: of the whole batch), are the rows of one
+// matrix.  A block takes a tile of 8 NT of those rows and a chunk of keys; its warps take 32 (16) keys at a time in turn, each with a running
+// maximum and sum of its own, and join at the end; chunks (and the prefix) are joined by attend_join_kernel through the workspace.
+//
+// Products run on mma.m16n8k16 with the keys on the M side: S^T = K Q^T has 16 keys by 8 rows to an instruction, so the 8 query heads of
+// a key/value head fill it, and O^T = V^T P^T takes its second operand from S^T by one 8x8 transpose between lanes.  A lane's share of K and
+// of V^T is loaded from global memory straight into registers in 4 to 16-byte pieces that together cover whole sectors of the cache's rows: no
+// shared memory on the way, no barrier in the loop, the loads of the next keys fly while this step's values are multiplied.
+//   Keys: lane (r = lane / 4, c = lane % 4) holds keys r and r + 8 of a tile; any order of head_dim serves as the k index as long as Q has
+//   the same, so a lane's pieces are contiguous.  Values: it holds keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them by byte permutes.
+//
+// Precision.  The codes are whole numbers and go into the product exactly; the scales stay outside in fp32: a key's multiplies the score,
+// a value's the weight p.  Q8: codes as f16 (a byte under the exponent of 1024), queries as f16 with a power of two to a row that puts its
+// largest value at 2^14 (bf16 queries lose nothing that is above 2^-28 of the row's largest; fp32 ones are split in two), weights times scales as f16
+// under a power of two that follows the largest scale seen.  Q4 and BF16: bf16 operands; fp32 queries and weights are split in three.
+// For bf16 queries the weights are one f16 (2^-11 of each) or two bf16 (2^-16).  Scores, maxima, sums and outputs are fp32; as the
+// instruction's accumulator drops what falls below its last bit, fp32 queries add its short runs up in fp32 proper.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "context.cuh"
+#include "kv_cache.cuh"
+
+namespace b200moe {
+
+struct AttnParams {
+    KvView kv;
+    const char * q;
+    char * out;
+    float * lse;                                     // [n_tokens][n_head] or null
+    int64_t q_token, q_head, out_token, out_head;    // strides in bytes
+    int n_tokens, n_head, group;                     // group: query heads to a key/value head
+    int n_seq, max_new, max_kv_len, prefix_len, pages_stride;
+    const int32_t * q_start;                         // [n_seq + 1]; null: one token to a sequence
+    const int32_t * kv_len;
+    const int32_t * pages;                           // [n_seq][pages_stride]
+    const int32_t * prefix_pages;
+    float scale_log2;                                // scale * log2(e)
+    int own_chunk, own_chunks;                       // keys to a chunk, most chunks of a sequence (0: there are no own keys)
+    int prefix_chunk, prefix_chunks;
+    int row_tiles;                                   // of the launch: tiles of rows per sequence (own) or of the whole batch (prefix)
+    int direct;                                      // one chunk in all: the block writes the result itself
+    float * part_o;                                  // [n_tokens * n_head][chunks][D]
+    float2 * part_ml;                                // [n_tokens * n_head][chunks]: maximum (of log2), sum
+    int * err;
+};
+
+// rows of sequence b; false (and the error word set) where the lengths are not what the arguments allow
+__device__ __forceinline__ bool attn_sequence(const AttnParams & p, int b, int & first, int & n_new, int & len, bool report) {
+    first = p.q_start ? p.q_start[b] : b;
+    const int next = p.q_start ? p.q_start[b + 1] : b + 1;
+    n_new = next - first;
+    len = p.own_chunks ? p.kv_len[b] : 0;
+    if (first < 0 || next > p.n_tokens || n_new < 0 || n_new > p.max_new || len < 0 || len > p.max_kv_len) {
+        if (report) report_error(p.err, DEV_ERR_BAD_LENGTH);
+        return false;
+    }
+    return true;
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// two floats as the N terms of a sum of f16 / bf16 pairs: the first rounds the value, each further one what the ones before left
+template <bool BF16, int N>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&out)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (BF16) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+            out[n] = *reinterpret_cast<const uint32_t *>(&h);
+            if (n + 1 < N) { x -= __low2float(h); y -= __high2float(h); }
+        } else {
+            const __half2 h = __floats2half2_rn(x, y);
+            out[n] = *reinterpret_cast<const uint32_t *>(&h);
+            if (n + 1 < N) { x -= __low2float(h); y -= __high2float(h); }
+        }
+    }
+}
+
+__device__ __forceinline__ uint4 load_stream(const uint4 * p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load_stream(const uint2 * p) {
+    uint2 v;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_stream(const uint32_t * p) {
+    uint32_t v;
+    asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
+// bytes u (0 .. 255, in the two bytes that `sel` names) as the f16 pair u - 128
+__device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
+    const uint32_t h = __byte_perm(w, 0x64646464u, sel);    // 1024 + u
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+// the low nibbles of w's two 16-bit halves as the bf16 pair n - 8
+__device__ __forceinline__ uint32_t nibbles_to_bf162(uint32_t w) {
+    const uint32_t h = (w & 0x000f000fu) | 0x43004300u;     // 128 + n
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&h), __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+// The lane's share of a 16-key tile, as loaded; and what the products take from it.  KW, VW: 32-bit words of a key's row that a lane holds.
+template <int TYPE, int D>
+struct AttnTile {
+    static constexpr int KW = TYPE == KV_BF16 ? D / 8 : TYPE == KV_Q8 ? D / 16 : D / 32;    // a quarter of a row
+    static constexpr int VW = KW / 2;                                                       // an eighth
+    static constexpr int RB = kv_row_bytes<TYPE, D>();
+    static constexpr int G = TYPE == KV_Q4 ? D / 32 : 1;                                    // scales to a row
+    static constexpr int KP = KW >= 4 ? 4 : 2;                                              // words to a load
+    static constexpr int VP = TYPE == KV_BF16 ? 4 : VW >= 2 ? 2 : 1;
+};
+
+template <int TYPE, int D>
+struct KeyRegs {
+    typedef AttnTile<TYPE, D> A;
+    uint32_t w[2][A::KW];
+    float d[2][A::G];    // scales (Q8 as they are; Q4 widened when used)
+};
+
+template <int TYPE, int D>
+__device__ __forceinline__ void load_scales(float (&d)[AttnTile<TYPE, D>::G], const void * scales, int64_t row) {
+    if (TYPE == KV_Q8) {
+        d[0] = static_cast<const float *>(scales)[row];
+    } else if (TYPE == KV_Q4) {
+        constexpr int G = AttnTile<TYPE, D>::G;
+        const uint32_t * p = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(scales) + row * G);
+#pragma unroll
+        for (int g = 0; g < G; g += 2) {
+            const uint32_t w = p[g / 2];
+            d[g] = __uint_as_float(w << 16);
+            d[(g + 1) % G] = __uint_as_float(w & 0xffff0000u);
+        }
+    }
+}
+
+template <int TYPE, int D>
+__device__ __forceinline__ void load_keys(KeyRegs<TYPE, D> & t, const KvView & kv, int64_t row0, int lane) {
+    typedef AttnTile<TYPE, D> A;
+    const int r = lane / 4, c = lane % 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t row = row0 + r + 8 * i;
+        const uint8_t * at = kv.k + row * A::RB;
+#pragma unroll
+        for (int w = 0; w < A::KW; w += A::KP) {
+            // pieces of the four lanes lie side by side
+            if constexpr (A::KP == 4) {
+                const uint4 v = load_stream(reinterpret_cast<const uint4 *>(at + 16 * w + 16 * c));
+                t.w[i][w] = v.x; t.w[i][w + 1] = v.y; t.w[i][w + 2] = v.z; t.w[i][w + 3] = v.w;
+            } else {
+                const uint2 v = load_stream(reinterpret_cast<const uint2 *>(at + 16 * w + 8 * c));
+                t.w[i][w] = v.x; t.w[i][w + 1] = v.y;
+            }
+        }
+        load_scales<TYPE, D>(t.d[i], kv.k_scale, row);
+    }
+}
+
+template <int TYPE, int D>
+struct ValueRegs {
+    typedef AttnTile<TYPE, D> A;
+    uint32_t w[4][A::VW];    // keys 2c, 2c + 1, 2c + 8, 2c + 9
+    float d[2][A::G];        // scales of keys r and r + 8, which the weights take on before they are transposed
+};
+
+template <int TYPE, int D>
+__device__ __forceinline__ void load_values(ValueRegs<TYPE, D> & t, const KvView & kv, int64_t row0, int lane) {
+    typedef AttnTile<TYPE, D> A;
+    const int r = lane / 4, c = lane % 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + 2 * c + (i & 1) + 8 * (i >> 1);
+        const uint8_t * at = kv.v + row * A::RB;
+#pragma unroll
+        for (int w = 0; w < A::VW; w += A::VP) {
+            const uint8_t * piece = at + 32 * w + 4 * A::VP * r;
+            if constexpr (A::VP == 4) {
+                const uint4 v = load_stream(reinterpret_cast<const uint4 *>(piece));
+                t.w[i][w] = v.x; t.w[i][w + 1] = v.y; t.w[i][w + 2] = v.z; t.w[i][w + 3] = v.w;
+            } else if constexpr (A::VP == 2) {
+                const uint2 v = load_stream(reinterpret_cast<const uint2 *>(piece));
+                t.w[i][w] = v.x; t.w[i][w + 1] = v.y;
+            } else {
+                t.w[i][w] = load_stream(reinterpret_cast<const uint32_t *>(piece));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) load_scales<TYPE, D>(t.d[i], kv.v_scale, row0 + r + 8 * i);
+}
+
+// Operand A of the score product's k step: 16 keys by the 16 head_dim indexes key_dim() names
+template <int TYPE, int D>
+__device__ __forceinline__ void key_operand(uint32_t (&a)[4], const KeyRegs<TYPE, D> & t, int step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (TYPE == KV_BF16) {
+            a[i] = t.w[i][2 * step];
+            a[2 + i] = t.w[i][2 * step + 1];
+        } else if (TYPE == KV_Q8) {
+            a[i] = bytes_to_half2(t.w[i][step], 0x4140);
+            a[2 + i] = bytes_to_half2(t.w[i][step], 0x4342);
+        } else {
+            const uint32_t w = t.w[i][step / 2] >> (step & 1 ? 8 : 0);
+            a[i] = nibbles_to_bf162(w);
+            a[2 + i] = nibbles_to_bf162(w >> 4);
+        }
+    }
+}
+// head_dim index of k step `step`, lane column c, value v: 0, 1 are the pair of the operand's first 8 columns, 2, 3 of the last
+template <int TYPE, int D>
+__device__ __forceinline__ int key_dim(int step, int c, int v) {
+    if (TYPE == KV_BF16) return 32 * (step / 2) + 8 * c + 4 * (step & 1) + v;
+    if (TYPE == KV_Q8) return 64 * (step / 4) + 16 * c + 4 * (step & 3) + v;
+    return 32 * (step / 2) + 8 * c + 2 * (step & 1) + (v >> 1) + 4 * (v & 1);
+}
+
+// Operand A of the output product's m tile: 16 head_dim indexes by 16 keys; lane row r is index value_dim(), row r + 8 the one behind it
+template <int TYPE, int D>
+__device__ __forceinline__ void value_operand(uint32_t (&a)[4], const ValueRegs<TYPE, D> & t, int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {    // keys 2c, 2c + 1, then 2c + 8, 2c + 9
+        if (TYPE == KV_BF16) {
+            const uint32_t x = t.w[2 * i][tile], y = t.w[2 * i + 1][tile];
+            a[2 * i] = __byte_perm(x, y, 0x5410);
+            a[2 * i + 1] = __byte_perm(x, y, 0x7632);
+        } else if (TYPE == KV_Q8) {
+            const uint32_t w = __byte_perm(t.w[2 * i][tile / 2], t.w[2 * i + 1][tile / 2], tile & 1 ? 0x7362 : 0x5140);
+            a[2 * i] = bytes_to_half2(w, 0x4140);
+            a[2 * i + 1] = bytes_to_half2(w, 0x4342);
+        } else {
+            const uint32_t w = __byte_perm(t.w[2 * i][tile / 4], t.w[2 * i + 1][tile / 4], tile & 2 ? 0x7632 : 0x5410) >> (tile & 1 ? 8 : 0);
+            a[2 * i] = nibbles_to_bf162(w);
+            a[2 * i + 1] = nibbles_to_bf162(w >> 4);
+        }
+    }
+}
+template <int TYPE, int D>
+__device__ __forceinline__ int value_dim(int tile, int r) {
+    if (TYPE == KV_Q4) return 32 * (tile / 2) + 4 * r + 2 * (tile & 1);
+    return 64 * (tile / 4) + 8 * r + 2 * (tile & 3);
+}
+
+constexpr int ATTN_WARPS = 4;
+
+template <int TYPE, int D, typename XT, int NT>
+struct AttnShape {
+    static constexpr bool F32 = sizeof(XT) == 4;
+    static constexpr bool BF = TYPE != KV_Q8;                                      // operands in bf16, else f16
+    static constexpr int QT = F32 ? (BF ? 3 : 2) : 1;                              // terms of a query
+    static constexpr int PT = F32 ? (BF ? 3 : 2) : (BF ? 2 : 1);                   // terms of a weight
+    static constexpr int STEPS = D / 16;                                           // k steps of the scores, m tiles of the outputs
+    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? 2 : 1;    // 16-key tiles to a pass of a warp
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int Q_WORDS = QT * STEPS * NT * 64;
+    static constexpr size_t SMEM_Q = Q_WORDS * 4 + ROWS * 8;                       // operands, then factor and reach of every row
+    static constexpr size_t SMEM_O = (size_t) ATTN_WARPS * ROWS * (D + 2) * 4;     // outputs, maxima and sums of the warps
+    static constexpr size_t SMEM = SMEM_Q > SMEM_O ? SMEM_Q : SMEM_O;
+};
+
+// PREFIX: rows are those of the whole batch and keys the prefix's; else blocks belong to a sequence
+template <int TYPE, int D, typename XT, int NT, bool PREFIX>
+__global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_constant__ AttnParams p) {
+    typedef AttnShape<TYPE, D, XT, NT> S;
+    typedef AttnTile<TYPE, D> A;
+    extern __shared__ __align__(16) uint32_t smem[];
+    uint32_t * sq = smem;
+    float * s_factor = reinterpret_cast<float *>(smem + S::Q_WORDS);
+    int * s_seen = reinterpret_cast<int *>(s_factor + S::ROWS);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
+    // row tiles of one chunk are neighbours, so that they share its keys in L2
+    int at = blockIdx.x;
+    const int row_tile = at % p.row_tiles;
+    at /= p.row_tiles;
+    const int head = at % p.kv.n_head;
+    at /= p.kv.n_head;
+    const int chunk = PREFIX ? at : at % p.own_chunks;
+    const int seq = PREFIX ? 0 : at / p.own_chunks;
+
+    // The prefix's kernel lets the own keys' kernel start beside it.  That one reads nothing that the first writes; its block 0 waits for the
+    // first to be done, so that what waits for the second waits for both.
+    if (PREFIX) pdl_launch_dependents();
+    else if (blockIdx.x == 0) pdl_wait();
+    int first = 0, n_new, len;
+    if (PREFIX) {
+        n_new = min(max(p.q_start ? p.q_start[p.n_seq] : p.n_seq, 0), p.n_tokens);
+        len = p.prefix_len;
+    } else if (!attn_sequence(p, seq, first, n_new, len, threadIdx.x == 0 && row_tile == 0 && head == 0 && chunk == 0)) {
+        return;
+    }
+    const int row0 = row_tile * S::ROWS, n_rows = min(n_new * p.group - row0, S::ROWS);
+    const int key0 = chunk * (PREFIX ? p.prefix_chunk : p.own_chunk);
+    if (n_rows <= 0 || (key0 >= len && !(key0 == 0 && p.direct))) return;
+    // keys that a row sees
+    auto reach = [&](int row) { return PREFIX ? len : max(0, len - n_new + (row0 + row) / p.group + 1); };
+    const int key_end = min(key0 + (PREFIX ? p.prefix_chunk : p.own_chunk), reach(n_rows - 1));
+    const int seen_by_all = reach(0);
+
+    // the queries as operands, a row at a time per warp
+    for (int row = warp; row < S::ROWS; row += ATTN_WARPS) {
+        const bool there = row < n_rows;
+        const int token = there ? first + (row0 + row) / p.group : 0, h = there ? head * p.group + (row0 + row) % p.group : 0;
+        const XT * src = reinterpret_cast<const XT *>(p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head);
+        float up = 1.0f, factor = p.scale_log2;
+        if (!S::BF) {
+            float m = 0.0f;
+            if (there)
+                for (int i = lane; i < D; i += 32) m = fmaxf(m, fabsf(to_float(src[i])));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int e = min(max((int) (__float_as_uint(m) >> 23), 40), 250);    // 2^(e - 127) <= m, kept where both powers are normal
+            up = __uint_as_float((uint32_t) (254 + 14 - e) << 23);
+            factor = p.scale_log2 / up;
+        }
+        if (lane == 0) {
+            s_factor[row] = factor;
+            s_seen[row] = there ? reach(row) : 0;
+        }
+        // word (term, step, row / 8, lane, half) of the operand; lane (row % 8, c)
+        for (int e = lane; e < S::STEPS * 8; e += 32) {
+            const int half = e & 1, cc = (e >> 1) & 3, step = e >> 3;
+            float x = 0.0f, y = 0.0f;
+            if (there) {
+                x = to_float(src[key_dim<TYPE, D>(step, cc, 2 * half)]) * up;
+                y = to_float(src[key_dim<TYPE, D>(step, cc, 2 * half + 1)]) * up;
+            }
+            uint32_t terms[S::QT];
+            split2<S::BF, S::QT>(x, y, terms);
+#pragma unroll
+            for (int n = 0; n < S::QT; ++n) sq[(((n * S::STEPS + step) * NT + row / 8) * 32 + (row % 8) * 4 + cc) * 2 + half] = terms[n];
+        }
+    }
+    __syncthreads();
+    float factor[NT][2];
+    int seen[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            factor[n][i] = s_factor[8 * n + 2 * c + i];
+            seen[n][i] = s_seen[8 * n + 2 * c + i];
+        }
+
+    float o[S::STEPS][NT][4], m[NT][2], l[NT][2];
+    int top[NT][2];    // Q8: exponent bits of the largest value scale that the row has seen, 2^-100 at least
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { m[n][i] = -INFINITY; l[n][i] = 0.0f; top[n][i] = 27 << 23; }
+#pragma unroll
+    for (int t = 0; t < S::STEPS; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][n][i] = 0.0f;
+
+    const int32_t * table = PREFIX ? p.prefix_pages : p.pages + (int64_t) seq * p.pages_stride;
+    const int shift = p.kv.page_shift, in_page = (1 << shift) - 1, n_pages = (int) (p.kv.n_slots >> shift);
+    constexpr int STRIDE = 16 * S::KS * ATTN_WARPS;
+    // first cache row of a 16-key tile (a page is a whole number of tiles); a page that the cache does not have is reported, its keys count as unseen
+    auto tile_page = [&](int key) { return key < key_end ? table[key >> shift] : 0; };
+    auto tile_row = [&](int page, int key) { return (((int64_t) page * p.kv.n_head + head) << shift) + (key & in_page); };
+    KeyRegs<TYPE, D> kr[S::KS];
+    ValueRegs<TYPE, D> vr[S::KS];
+    int page[S::KS], next_page[S::KS];
+    bool good[S::KS];
+    int key = key0 + warp * 16 * S::KS;
+#pragma unroll
+    for (int j = 0; j < S::KS; ++j) page[j] = tile_page(key + 16 * j);
+#pragma unroll
+    for (int j = 0; j < S::KS; ++j) next_page[j] = tile_page(key + STRIDE + 16 * j);
+    auto check = [&](int j) {
+        good[j] = page[j] >= 0 && page[j] < n_pages;
+        if (!good[j]) {
+            if (lane == 0) report_error(p.err, DEV_ERR_BAD_SLOT);
+            page[j] = 0;
+        }
+    };
+    if (key < key_end) {
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) {
+            check(j);
+            const int64_t row = tile_row(page[j], key + 16 * j);
+            load_keys<TYPE, D>(kr[j], p.kv, row, lane);
+            load_values<TYPE, D>(vr[j], p.kv, row, lane);
+        }
+    }
+    for (; key < key_end; key += STRIDE) {
+        // ---- scores: 16 keys by 8 NT rows; lane has keys r, r + 8 and rows 2c, 2c + 1
+        float s[S::KS][NT][4];
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[j][n][i] = 0.0f;
+        constexpr int RUN = S::F32 ? 2 : S::STEPS / A::G;    // k steps summed in the instruction's accumulator
+#pragma unroll
+        for (int run = 0; run < S::STEPS / RUN; ++run) {
+            const int g = run * RUN * A::G / S::STEPS;
+            float part[S::KS][NT][4];
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[j][n][i] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < RUN; ++u) {
+                const int step = run * RUN + u;
+                uint32_t a[S::KS][4];
+#pragma unroll
+                for (int j = 0; j < S::KS; ++j) key_operand<TYPE, D>(a[j], kr[j], step);
+#pragma unroll
+                for (int term = 0; term < S::QT; ++term)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const uint2 b = *reinterpret_cast<const uint2 *>(sq + (((term * S::STEPS + step) * NT + n) * 32 + lane) * 2);
+#pragma unroll
+                        for (int j = 0; j < S::KS; ++j) mma16816<S::BF>(part[j][n], a[j][0], a[j][1], a[j][2], a[j][3], b.x, b.y);
+                    }
+            }
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[j][n][i] = TYPE == KV_BF16 ? s[j][n][i] + part[j][n][i] : fmaf(part[j][n][i], kr[j].d[i >> 1][g], s[j][n][i]);
+        }
+        bool masked = key + 16 * S::KS > seen_by_all || key + 16 * S::KS > key_end;
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) masked |= !good[j];
+        bool was_good[S::KS];
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) was_good[j] = good[j];
+        // ---- the next keys fly from here on
+        const int next = key + STRIDE;
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) {
+            page[j] = next_page[j];
+            next_page[j] = tile_page(next + STRIDE + 16 * j);
+        }
+        if (next < key_end) {
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j) {
+                check(j);
+                load_keys<TYPE, D>(kr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
+            }
+        }
+        // ---- softmax
+        bool on[S::KS][NT][4];
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = key + 16 * j + r + 8 * (i >> 1);
+                        on[j][n][i] = was_good[j] && k < key_end && k < seen[n][i & 1];
+                        s[j][n][i] = on[j][n][i] ? s[j][n][i] * factor[n][i & 1] : -INFINITY;
+                    }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { on[j][n][i] = true; s[j][n][i] *= factor[n][i & 1]; }
+        }
+        bool grew = false;
+        float m_new[NT][2];
+        int top_new[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v = m[n][i];
+                int t = top[n][i];
+#pragma unroll
+                for (int j = 0; j < S::KS; ++j) {
+                    v = fmaxf(v, fmaxf(s[j][n][i], s[j][n][i + 2]));
+                    if (TYPE == KV_Q8) {    // NaN scales say nothing here, they make the weight NaN
+                        const float d0 = fabsf(vr[j].d[0][0]), d1 = fabsf(vr[j].d[1][0]);
+                        if (on[j][n][i] && d0 <= 3.4e38f) t = max(t, __float_as_int(d0) & 0x7f800000);
+                        if (on[j][n][i + 2] && d1 <= 3.4e38f) t = max(t, __float_as_int(d1) & 0x7f800000);
+                    }
+                }
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) {
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+                    if (TYPE == KV_Q8) t = max(t, __shfl_xor_sync(0xffffffffu, t, x));
+                }
+                m_new[n][i] = v;
+                top_new[n][i] = t;
+                grew |= v > m[n][i] || t > top[n][i];
+            }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float back[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    // nothing seen yet: no sum to scale back
+                    back[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - m_new[n][i]);
+                    l[n][i] *= back[i];
+                    if (TYPE == KV_Q8) {
+                        const int down = (top_new[n][i] - top[n][i]) >> 23;
+                        back[i] *= down > 126 ? 0.0f : __uint_as_float((uint32_t) (127 - down) << 23);
+                    }
+                    m[n][i] = m_new[n][i];
+                    top[n][i] = top_new[n][i];
+                }
+#pragma unroll
+                for (int t = 0; t < S::STEPS; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[t][n][i] *= back[i & 1];
+            }
+        }
+        // ---- outputs: 16 head_dim indexes by 8 NT rows
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) {
+            float w[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float base = m[n][i & 1] == -INFINITY ? 0.0f : m[n][i & 1];
+                    w[n][i] = fast_exp2(s[j][n][i] - base);
+                    l[n][i & 1] += w[n][i];
+                }
+            uint32_t b[S::PT][NT][2];
+            bool poison = false;
+            if (TYPE == KV_BF16 && masked) {
+                // a value that some rows do not see must not reach them as 0 times infinity
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int x = 0; x < A::VW; ++x) {
+                        const uint32_t v = vr[j].w[i][x];
+                        poison |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+                    }
+                poison = __any_sync(0xffffffffu, poison);
+            }
+#pragma unroll
+            for (int t = 0; t < S::STEPS; ++t) {
+                if (t % (S::STEPS / A::G) == 0) {    // the weights times the scales of this group
+                    const int g = t / (S::STEPS / A::G);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float x[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = w[n][i];
+                            if (TYPE == KV_Q8) {    // w * d * 2^(13 - exponent of top) < 2^14
+                                const float norm = __uint_as_float(((254u + 13u) << 23) - (uint32_t) top[n][i & 1]);
+                                x[i] = on[j][n][i] ? w[n][i] * (vr[j].d[i >> 1][0] * norm) : 0.0f;
+                            } else if (TYPE == KV_Q4) {
+                                x[i] = on[j][n][i] ? w[n][i] * vr[j].d[i >> 1][g] : 0.0f;
+                            }
+                        }
+                        uint32_t lo[S::PT], hi[S::PT];
+                        split2<S::BF, S::PT>(x[0], x[1], lo);
+                        split2<S::BF, S::PT>(x[2], x[3], hi);
+#pragma unroll
+                        for (int u = 0; u < S::PT; ++u) {
+                            b[u][n][0] = transpose8x8(lo[u]);
+                            b[u][n][1] = transpose8x8(hi[u]);
+                        }
+                    }
+                }
+                uint32_t a[4];
+                value_operand<TYPE, D>(a, vr[j], t);
+                if (TYPE == KV_BF16 && poison) {
+                    // 1 where the value is not finite: its product with the rows that see the key says whose output it spoils
+                    uint32_t bad[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool x = (a[i] & 0x7f80u) == 0x7f80u, y = (a[i] & 0x7f800000u) == 0x7f800000u;
+                        bad[i] = (x ? 0x3f80u : 0u) | (y ? 0x3f800000u : 0u);
+                        a[i] &= (x ? 0u : 0xffffu) | (y ? 0u : 0xffff0000u);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float spoilt[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                        const uint32_t see0 = transpose8x8((on[j][n][0] ? 0x3f80u : 0u) | (on[j][n][1] ? 0x3f800000u : 0u));
+                        const uint32_t see1 = transpose8x8((on[j][n][2] ? 0x3f80u : 0u) | (on[j][n][3] ? 0x3f800000u : 0u));
+                        mma16816<true>(spoilt, bad[0], bad[1], bad[2], bad[3], see0, see1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (spoilt[i] > 0.0f) o[t][n][i] = __uint_as_float(0x7fffffffu);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float part[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                    for (int u = S::PT - 1; u >= 0; --u)
+                        mma16816<S::BF>(S::F32 ? part : o[t][n], a[0], a[1], a[2], a[3], b[u][n][0], b[u][n][1]);
+                    if (S::F32)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[t][n][i] += part[i];
+                }
+            }
+        }
+        if (next < key_end) {
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j) load_values<TYPE, D>(vr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
+        }
+    }
+
+    // ---- join the warps
+    if (!PREFIX) pdl_launch_dependents();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+    __syncthreads();    // the operands are done with
+    float * so = reinterpret_cast<float *>(smem);
+    float2 * sml = reinterpret_cast<float2 *>(so + (size_t) ATTN_WARPS * S::ROWS * D);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        float unit[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            unit[i] = TYPE == KV_Q8 ? __uint_as_float((uint32_t) top[n][i] - (13u << 23)) : 1.0f;
+#pragma unroll
+        for (int t = 0; t < S::STEPS; ++t) {
+            const int d = value_dim<TYPE, D>(t, r);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float2 v = make_float2(o[t][n][i] * unit[i], o[t][n][i + 2] * unit[i]);
+                *reinterpret_cast<float2 *>(so + ((size_t) warp * S::ROWS + 8 * n + 2 * c + i) * D + d) = v;
+            }
+        }
+        if (r == 0)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sml[warp * S::ROWS + 8 * n + 2 * c + i] = make_float2(m[n][i], l[n][i]);
+    }
+    __syncthreads();
+    const int chunks = p.prefix_chunks + p.own_chunks, slot = PREFIX ? chunk : p.prefix_chunks + chunk;
+    for (int e = threadIdx.x; e < n_rows * (D / 2); e += 32 * ATTN_WARPS) {
+        const int row = e / (D / 2), d = 2 * (e % (D / 2));
+        float most = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ATTN_WARPS; ++w) most = fmaxf(most, sml[w * S::ROWS + row].x);
+#pragma unroll
+        for (int w = 0; w < ATTN_WARPS; ++w) {
+            const float2 ml = sml[w * S::ROWS + row];
+            const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - most);
+            const float2 v = *reinterpret_cast<const float2 *>(so + ((size_t) w * S::ROWS + row) * D + d);
+            if (ml.x != -INFINITY || ml.y != 0.0f) { sum += ml.y * f; x += v.x * f; y += v.y * f; }
+        }
+        const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
+        const int64_t line = (int64_t) token * p.n_head + h;
+        if (p.direct) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            XT * dst = reinterpret_cast<XT *>(p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head) + d;
+            dst[0] = from_float<XT>(x * inv);
+            dst[1] = from_float<XT>(y * inv);
+            if (p.lse && d == 0) p.lse[line] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
+        } else {
+            *reinterpret_cast<float2 *>(p.part_o + (line * chunks + slot) * D + d) = make_float2(x, y);
+            if (d == 0) p.part_ml[line * chunks + slot] = make_float2(most, sum);
+        }
+    }
+}
+
+// joins the chunks of a (token, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c
+template <int D, typename XT>
+__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int WARPS = 4, PER = D / 32;
+    __shared__ float so[WARPS][D];
+    __shared__ float2 sml[WARPS];
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t line = blockIdx.x;
+    const int token = (int) (line / p.n_head);
+    int seq = token;
+    if (p.q_start) {    // the last sequence that begins at or before the token
+        int low = 0, high = p.n_seq;
+        while (high - low > 1) {
+            const int mid = (low + high) / 2;
+            if (p.q_start[mid] <= token) low = mid;
+            else high = mid;
+        }
+        seq = low;
+    }
+    int first, n_new, len;
+    if (seq >= p.n_seq || !attn_sequence(p, seq, first, n_new, len, false) || token < first || token >= first + n_new) return;    // a row that belongs to nobody
+    const int reach = max(0, len - n_new + (token - first) + 1);
+    const int own = p.own_chunks ? (reach + p.own_chunk - 1) / p.own_chunk : 0;
+    const int n = p.prefix_chunks + own, chunks = p.prefix_chunks + p.own_chunks;
+    const float2 * ml = p.part_ml + line * chunks;
+    const float * o = p.part_o + line * chunks * D;
+    float most = -INFINITY;
+    for (int i = lane; i < n; i += 32) most = fmaxf(most, ml[i].x);
+#pragma unroll
+    for (int x = 16; x > 0; x /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+    float acc[PER], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int i = warp; i < n; i += WARPS) {
+        const float2 x = ml[i];
+        const float f = x.x == -INFINITY ? 0.0f : fast_exp2(x.x - most);
+        const Pack<float, PER> v = *reinterpret_cast<const Pack<float, PER> *>(o + (int64_t) i * D + lane * PER);
+        if (x.x != -INFINITY || x.y != 0.0f) {
+            sum += x.y * f;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) acc[j] += v.v[j] * f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) so[warp][lane * PER + j] = acc[j];
+    if (lane == 0) sml[warp] = make_float2(most, sum);
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += sml[w].y;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int h = (int) (line % p.n_head);
+    XT * dst = reinterpret_cast<XT *>(p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head);
+    for (int d = threadIdx.x; d < D; d += 128) {
+        float x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) x += so[w][d];
+        dst[d] = from_float<XT>(x * inv);
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[line] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
+}
+
+// One launch for the own keys or the prefix; the kernels are in a translation unit for each type of cache.  nt: rows to a tile / 8, 1, 2 or 4
+// (at most attend_tiles()); overlap: the own keys' kernel starts beside the prefix's.
+template <int TYPE>
+int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st);
+
+// most rows to a tile / 8: what leaves the outputs and the loads in registers
+inline int attend_tiles(int head_dim, bool f32) { return f32 || head_dim == 256 ? 2 : 4; }
+
+}  // namespace b200moe

@@ -1,0 +1,57 @@
+// Launches of the attention kernels for one type of cache; included by that type's translation unit alone.
+#pragma once
+#include "attention.cuh"
+
+namespace b200moe {
+
+constexpr int ATTN_MAX_DEVICES = 64;
+
+template <int TYPE, int D, typename XT, int NT, bool PREFIX>
+int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int blocks, cudaStream_t st) {
+    auto kern = attend_kernel<TYPE, D, XT, NT, PREFIX>;
+    constexpr size_t smem = AttnShape<TYPE, D, XT, NT>::SMEM;
+    if (smem > 48 * 1024) {    // an attribute of the (function, device) pair
+        static bool done[ATTN_MAX_DEVICES] = {};
+        if (ctx->device >= ATTN_MAX_DEVICES) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "device ordinal %d out of range", ctx->device);
+        if (!done[ctx->device]) {
+            CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+            done[ctx->device] = true;
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) blocks);
+    cfg.blockDim = dim3(32 * ATTN_WARPS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, p));
+    return check_launch(ctx, "attention");
+}
+
+template <int TYPE, int D, typename XT, bool PREFIX>
+int launch_attend_n(ContextBase * ctx, const AttnParams & p, int nt, bool overlap, int blocks, cudaStream_t st) {
+    if (nt == 1) return launch_attend_t<TYPE, D, XT, 1, PREFIX>(ctx, p, overlap, blocks, st);
+    if (nt == 2) return launch_attend_t<TYPE, D, XT, 2, PREFIX>(ctx, p, overlap, blocks, st);
+    if constexpr (D < 256 && sizeof(XT) == 2) return launch_attend_t<TYPE, D, XT, 4, PREFIX>(ctx, p, overlap, blocks, st);
+    return fail(ctx, B200MOE_ERR_UNSUPPORTED, "no kernel for %d rows to a tile", 8 * nt);
+}
+
+template <int TYPE, int D>
+int launch_attend_d(ContextBase * ctx, const AttnParams & p, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st) {
+    if (f32) return prefix ? launch_attend_n<TYPE, D, float, true>(ctx, p, nt, overlap, blocks, st) : launch_attend_n<TYPE, D, float, false>(ctx, p, nt, overlap, blocks, st);
+    return prefix ? launch_attend_n<TYPE, D, __nv_bfloat16, true>(ctx, p, nt, overlap, blocks, st)
+                  : launch_attend_n<TYPE, D, __nv_bfloat16, false>(ctx, p, nt, overlap, blocks, st);
+}
+
+template <int TYPE>
+int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st) {
+    if (head_dim == 64) return launch_attend_d<TYPE, 64>(ctx, p, f32, nt, prefix, overlap, blocks, st);
+    if (head_dim == 128) return launch_attend_d<TYPE, 128>(ctx, p, f32, nt, prefix, overlap, blocks, st);
+    return launch_attend_d<TYPE, 256>(ctx, p, f32, nt, prefix, overlap, blocks, st);
+}
+
+}  // namespace b200moe

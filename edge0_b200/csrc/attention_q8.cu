@@ -1,0 +1,8 @@
+// attention over caches of type KV_Q8
+#include "attention_launch.cuh"
+
+namespace b200moe {
+
+template int launch_attend<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+
+}  // namespace b200moe

@@ -7,7 +7,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -16,6 +15,7 @@
 #include <vector>
 
 #include "../../include/edge0_b200_moe.h"
+#include "context.cuh"
 #include "expert_gemm.cuh"
 #include "expert_gemm_fp4.cuh"
 #include "expert_exchange.cuh"
@@ -71,16 +71,10 @@ struct Plan {  // carved out of the scratch arena for one (layer shape, max_toke
 
 }  // namespace
 
-struct b200moe_ctx {
-    int device = 0;
-    int sm_count = 0;
+struct b200moe_ctx : ContextBase {
     Scratch scratch;
     Plan plan;
-    int * d_err = nullptr;  // 16 bytes: [error code][pad][fix-up overflow counter, 64 bit]
-    int * h_err = nullptr;  // pinned copy of the same
-    std::string last_error;
     b200moe_counters counters{};
-    int64_t launches = 0;
     bool timing = false;
     int expert_path = 0;  // b200moe_set_expert_path
     bool overlap = true;       // b200moe_set_launch_overlap (see layer_overlap)
@@ -91,25 +85,9 @@ struct b200moe_ctx {
     std::vector<Timed> timed;
 };
 
+b200moe::ContextBase * b200moe::context_base(b200moe_ctx * ctx) { return ctx; }
+
 namespace {
-
-int fail(b200moe_ctx * ctx, int code, const char * fmt, ...) {
-    if (ctx) {
-        char buf[512];
-        va_list ap;
-        va_start(ap, fmt);
-        vsnprintf(buf, sizeof buf, fmt, ap);
-        va_end(ap);
-        ctx->last_error = buf;
-    }
-    return code;
-}
-
-#define CUDA_TRY(ctx, expr)                                                                          \
-    do {                                                                                             \
-        cudaError_t _e = (expr);                                                                     \
-        if (_e != cudaSuccess) return fail(ctx, B200MOE_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(_e)); \
-    } while (0)
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
@@ -321,13 +299,6 @@ int raise_smem_limit(b200moe_ctx * ctx, Kern kern, size_t smem, bool (&done)[MAX
         CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
         done[ctx->device] = true;
     }
-    return B200MOE_OK;
-}
-
-int check_launch(b200moe_ctx * ctx, const char * what) {
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(ctx, B200MOE_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
-    ctx->launches++;
     return B200MOE_OK;
 }
 
@@ -1042,7 +1013,8 @@ int read_device_error(b200moe_ctx * ctx, cudaStream_t st) {
     if (*ctx->h_err != 0) {
         const int code = *ctx->h_err;
         cudaMemsetAsync(ctx->d_err, 0, sizeof(int), st);
-        return fail(ctx, B200MOE_ERR_DEVICE_CHECK, "device check failed with code %d (1 barrier wait ran out, 2 expert id out of range, 3 shape)", code);
+        return fail(ctx, B200MOE_ERR_DEVICE_CHECK, "device check failed with code %d (1 barrier wait ran out, 2 expert id out of range, 3 shape, 4 cache slot or page out of range, "
+                    "5 sequence lengths that the call does not allow)", code);
     }
     return B200MOE_OK;
 }

@@ -15,6 +15,8 @@ enum DeviceError : int {
     DEV_ERR_BARRIER_TIMEOUT = 1,
     DEV_ERR_BAD_EXPERT_ID = 2,
     DEV_ERR_BAD_SHAPE = 3,
+    DEV_ERR_BAD_SLOT = 4,     // a cache slot or page that the cache does not have
+    DEV_ERR_BAD_LENGTH = 5,   // sequence lengths outside of what the call's arguments allow
 };
 
 __device__ __forceinline__ void report_error(int * flag, int code) {

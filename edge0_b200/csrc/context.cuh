@@ -1,0 +1,52 @@
+// What every translation unit of the library needs of a context: its device, its error text and the device's error words.  The part that
+// only the MoE path uses (scratch, plan, launch mode) is in capi.cu, which derives b200moe_ctx from this.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <string>
+
+#include "../../include/edge0_b200_moe.h"
+
+namespace b200moe {
+
+struct ContextBase {
+    int device = 0;
+    int sm_count = 0;
+    int * d_err = nullptr;  // 16 bytes: [error code][pad][fix-up overflow counter, 64 bit]
+    int * h_err = nullptr;  // pinned copy of the same
+    std::string last_error;
+    int64_t launches = 0;
+};
+
+// the base of a context, for the translation units that do not see the whole of it (null for null)
+ContextBase * context_base(b200moe_ctx * ctx);
+
+inline int fail(ContextBase * ctx, int code, const char * fmt, ...) {
+    if (ctx) {
+        char buf[512];
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(buf, sizeof buf, fmt, ap);
+        va_end(ap);
+        ctx->last_error = buf;
+    }
+    return code;
+}
+
+#define CUDA_TRY(ctx, expr)                                                                          \
+    do {                                                                                             \
+        cudaError_t _e = (expr);                                                                     \
+        if (_e != cudaSuccess) return fail(ctx, B200MOE_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(_e)); \
+    } while (0)
+
+inline int check_launch(ContextBase * ctx, const char * what) {
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(ctx, B200MOE_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+    ctx->launches++;
+    return B200MOE_OK;
+}
+
+}  // namespace b200moe

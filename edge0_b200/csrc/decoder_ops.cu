@@ -1,0 +1,342 @@
+// C ABI of the attention half of a decoder layer (include/edge0_b200_moe.h): argument checks, the split of the work, launches.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.cuh"
+#include "context.cuh"
+#include "kv_cache.cuh"
+#include "rope.cuh"
+
+using namespace b200moe;
+
+namespace {
+
+int elem_size(int type) { return type == B200MOE_TYPE_F32 ? 4 : type == B200MOE_TYPE_BF16 ? 2 : 0; }
+
+// [head_dim, heads, tokens] rows of x_type; `written`: rows that do not overlap
+int check_rows(ContextBase * ctx, const b200moe_tensor * t, int x_type, const char * what, bool written) {
+    const int64_t es = elem_size(x_type);
+    if (!t || !t->data) return fail(ctx, B200MOE_ERR_INVALID_ARG, "%s: null tensor", what);
+    if (t->ne[0] <= 0 || t->ne[1] <= 0 || t->ne[2] < 0 || t->ne[3] != 1)
+        return fail(ctx, B200MOE_ERR_INVALID_ARG, "%s: ne must be [head_dim, heads, tokens, 1]", what);
+    if (t->ne[0] > (1 << 20) || t->ne[1] > (1 << 20) || t->ne[2] >= ((int64_t) 1 << 31) || t->ne[1] * t->ne[2] >= ((int64_t) 1 << 31))
+        return fail(ctx, B200MOE_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (t->nb[0] != es || t->nb[1] < 0 || t->nb[2] < 0 || t->nb[1] % es || t->nb[2] % es || (uintptr_t) t->data % es)
+        return fail(ctx, B200MOE_ERR_INVALID_ARG, "%s: rows must be contiguous, strides whole elements and not negative", what);
+    if (written) {
+        int64_t low = t->nb[1], high = t->nb[2], n_low = t->ne[1], n_high = t->ne[2];
+        if (n_low == 1 || (n_high > 1 && high < low)) { std::swap(low, high); std::swap(n_low, n_high); }
+        if ((n_low > 1 && low < t->ne[0] * es) || (n_high > 1 && high < (n_low > 1 ? low * (n_low - 1) : 0) + t->ne[0] * es))
+            return fail(ctx, B200MOE_ERR_INVALID_ARG, "%s: rows that are written must not overlap", what);
+    }
+    return B200MOE_OK;
+}
+
+bool rows_aligned(const b200moe_tensor * t) { return !(((uintptr_t) t->data | (uintptr_t) t->nb[1] | (uintptr_t) t->nb[2]) & 15); }
+
+int row_bytes(int type, int d) { return type == KV_BF16 ? 2 * d : type == KV_Q8 ? d : d / 2; }
+int scale_row_bytes(int type, int d) { return type == KV_BF16 ? 0 : type == KV_Q8 ? 4 : 2 * (d / 32); }
+
+int check_cache_shape(ContextBase * ctx, const b200moe_kv_cache * c) {
+    if (!c) return fail(ctx, B200MOE_ERR_INVALID_ARG, "cache is null");
+    if (c->type < KV_BF16 || c->type > KV_Q4) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "cache type %d", c->type);
+    if (c->n_head_kv <= 0 || c->n_pages <= 0) return fail(ctx, B200MOE_ERR_INVALID_ARG, "non-positive cache dimension");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+        return fail(ctx, B200MOE_ERR_UNSUPPORTED, "page_size must be 16, 32, 64, 128 or 256");
+    if (c->n_head_kv > 65536 || c->n_pages > INT32_MAX / c->page_size) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "a cache has fewer than 2^31 slots");
+    return B200MOE_OK;
+}
+
+int check_cache(ContextBase * ctx, const b200moe_kv_cache * c, KvView & v) {
+    if (int rc = check_cache_shape(ctx, c)) return rc;
+    if (!c->k || !c->v || (c->type != KV_BF16 && (!c->k_scale || !c->v_scale))) return fail(ctx, B200MOE_ERR_INVALID_ARG, "null cache array");
+    if (((uintptr_t) c->k | (uintptr_t) c->v | (uintptr_t) c->k_scale | (uintptr_t) c->v_scale) & 15)
+        return fail(ctx, B200MOE_ERR_INVALID_ARG, "cache arrays must be 16-byte aligned");
+    v.k = static_cast<uint8_t *>(c->k);
+    v.v = static_cast<uint8_t *>(c->v);
+    v.k_scale = c->k_scale;
+    v.v_scale = c->v_scale;
+    v.n_slots = c->n_pages * c->page_size;
+    v.n_head = c->n_head_kv;
+    v.page_shift = 0;
+    while ((1 << v.page_shift) < c->page_size) ++v.page_shift;
+    return B200MOE_OK;
+}
+
+// ---- rotary positions
+template <typename T>
+int launch_rope(ContextBase * ctx, const RopeParams & p, bool adjacent, bool wide, cudaStream_t st) {
+    constexpr int VP = 16 / sizeof(T);
+    // a token's table of turns serves all its heads; a few tokens to a block where there are many, so that every thread has one to work out
+    const int half = p.n_rot / 2;
+    const int per_block = std::max(1, std::min({ ROPE_THREADS / half, p.n_tokens / (4 * ctx->sm_count), 8 }));
+    const int blocks = (p.n_tokens + per_block - 1) / per_block;
+    const size_t smem = sizeof(float2) * half * per_block;
+    if (smem > 48 * 1024) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "n_rot must be at most 12288");
+    if (wide && adjacent) rope_kernel<T, VP, true><<<blocks, ROPE_THREADS, smem, st>>>(p, per_block);
+    else if (wide) rope_kernel<T, VP, false><<<blocks, ROPE_THREADS, smem, st>>>(p, per_block);
+    else if (adjacent) rope_kernel<T, 1, true><<<blocks, ROPE_THREADS, smem, st>>>(p, per_block);
+    else rope_kernel<T, 1, false><<<blocks, ROPE_THREADS, smem, st>>>(p, per_block);
+    return check_launch(ctx, "rope");
+}
+
+// ---- cache
+template <int TYPE, int D, typename XT>
+int launch_kv(ContextBase * ctx, const KvView & c, const KvRows & x, const int32_t * slots, int64_t n_rows, bool write, cudaStream_t st) {
+    constexpr int ROWS = KV_THREADS / (D / 8);
+    const int64_t most = (int64_t) ctx->sm_count * 32;
+    const int blocks = (int) std::min<int64_t>((n_rows + ROWS - 1) / ROWS, most);
+    if (write) kv_write_kernel<TYPE, D, XT><<<blocks, KV_THREADS, 0, st>>>(c, x, slots, n_rows, ctx->d_err);
+    else kv_read_kernel<TYPE, D, XT><<<blocks, KV_THREADS, 0, st>>>(c, x, slots, n_rows, ctx->d_err);
+    return check_launch(ctx, write ? "kv_write" : "kv_read");
+}
+template <int TYPE, typename XT>
+int launch_kv_d(ContextBase * ctx, int d, const KvView & c, const KvRows & x, const int32_t * slots, int64_t n_rows, bool write, cudaStream_t st) {
+    if (d == 64) return launch_kv<TYPE, 64, XT>(ctx, c, x, slots, n_rows, write, st);
+    if (d == 128) return launch_kv<TYPE, 128, XT>(ctx, c, x, slots, n_rows, write, st);
+    return launch_kv<TYPE, 256, XT>(ctx, c, x, slots, n_rows, write, st);
+}
+template <typename XT>
+int launch_kv_t(ContextBase * ctx, int type, int d, const KvView & c, const KvRows & x, const int32_t * slots, int64_t n_rows, bool write, cudaStream_t st) {
+    if (type == KV_BF16) return launch_kv_d<KV_BF16, XT>(ctx, d, c, x, slots, n_rows, write, st);
+    if (type == KV_Q8) return launch_kv_d<KV_Q8, XT>(ctx, d, c, x, slots, n_rows, write, st);
+    return launch_kv_d<KV_Q4, XT>(ctx, d, c, x, slots, n_rows, write, st);
+}
+
+int kv_move(b200moe_ctx * c, const b200moe_kv_cache * cache, const b200moe_tensor * k, const b200moe_tensor * v, int x_type, const int32_t * slots,
+            bool write, void * stream) {
+    ContextBase * ctx = context_base(c);
+    if (!ctx) return B200MOE_ERR_INVALID_ARG;
+    KvView view;
+    if (int rc = check_cache(ctx, cache, view)) return rc;
+    if (!elem_size(x_type)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "rows must be F32 or BF16");
+    if (k && v && k->ne[2] == 0 && v->ne[2] == 0) return B200MOE_OK;
+    if (int rc = check_rows(ctx, k, x_type, "k", !write)) return rc;
+    if (int rc = check_rows(ctx, v, x_type, "v", !write)) return rc;
+    for (const b200moe_tensor * t : { k, v })
+        if (t->ne[0] != cache->head_dim || t->ne[1] != cache->n_head_kv || t->ne[2] != k->ne[2])
+            return fail(ctx, B200MOE_ERR_INVALID_ARG, "k and v must be [head_dim, n_head_kv, tokens] of the cache's head_dim and n_head_kv");
+    if (!slots) return fail(ctx, B200MOE_ERR_INVALID_ARG, "slots is null");
+    CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+    const KvRows x = { static_cast<char *>(k->data), static_cast<char *>(v->data), k->nb[2], k->nb[1], v->nb[2], v->nb[1], rows_aligned(k) && rows_aligned(v) };
+    const int64_t n_rows = k->ne[2] * cache->n_head_kv;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return x_type == B200MOE_TYPE_F32 ? launch_kv_t<float>(ctx, cache->type, cache->head_dim, view, x, slots, n_rows, write, st)
+                                      : launch_kv_t<__nv_bfloat16>(ctx, cache->type, cache->head_dim, view, x, slots, n_rows, write, st);
+}
+
+// ---- attention
+struct AttnPlan {
+    int own_nt, own_tiles, own_chunk, own_chunks;
+    int prefix_nt, prefix_tiles, prefix_chunk, prefix_chunks;
+    size_t part_o, bytes;
+};
+
+int tile_units(int64_t rows, int most) { return rows <= 8 ? 1 : rows <= 16 ? 2 : most; }
+
+// keys to a chunk, so that `base` blocks of whole length become about `blocks`
+void split_keys(int64_t len, int64_t base, int64_t blocks, int & chunk, int & chunks) {
+    constexpr int UNIT = 32 * ATTN_WARPS;    // a pass of every warp of a block
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((len + UNIT - 1) / UNIT, blocks / std::max<int64_t>(base, 1)));
+    chunk = (int) (((len + n - 1) / n + UNIT - 1) / UNIT * UNIT);
+    chunk = std::max(chunk, UNIT);
+    chunks = (int) ((len + chunk - 1) / chunk);
+}
+
+int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int64_t n_head, int64_t n_tokens) {
+    if (int rc = check_cache_shape(ctx, c)) return rc;
+    if (!a) return fail(ctx, B200MOE_ERR_INVALID_ARG, "attn is null");
+    if (a->n_seq < 0 || a->max_new < 0 || a->max_kv_len < 0 || a->prefix_len < 0 || a->pages_stride < 0 || n_head <= 0 || n_tokens < 0)
+        return fail(ctx, B200MOE_ERR_INVALID_ARG, "negative size, or no heads");
+    if (n_head % c->n_head_kv) return fail(ctx, B200MOE_ERR_INVALID_ARG, "n_head must be a multiple of n_head_kv");
+    if (!std::isfinite(a->scale)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "scale must be finite");
+    if ((int64_t) a->pages_stride * c->page_size < a->max_kv_len) return fail(ctx, B200MOE_ERR_INVALID_ARG, "max_kv_len needs more pages than a sequence's table has");
+    if (a->max_kv_len > INT32_MAX / 2 || a->prefix_len > INT32_MAX / 2) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "at most 2^30 positions");
+    if (n_tokens * n_head >= ((int64_t) 1 << 31) || (int64_t) a->max_new * n_head >= ((int64_t) 1 << 31)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
+    return B200MOE_OK;
+}
+
+int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int n_head, int n_tokens, bool f32, AttnPlan & pl) {
+    const int group = n_head / c->n_head_kv, most = attend_tiles(c->head_dim, f32);
+    const int64_t blocks = (int64_t) ctx->sm_count * 6;
+    pl = AttnPlan{};
+    const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group;
+    pl.own_nt = tile_units(own_rows, most);
+    pl.own_tiles = (int) ((own_rows + 8 * pl.own_nt - 1) / (8 * pl.own_nt));
+    split_keys(a->max_kv_len, (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, blocks, pl.own_chunk, pl.own_chunks);
+    pl.own_chunks = std::max(pl.own_chunks, 1);
+    if (a->prefix_len) {
+        const int64_t rows = (int64_t) n_tokens * group;
+        pl.prefix_nt = tile_units(rows, most);
+        pl.prefix_tiles = (int) ((rows + 8 * pl.prefix_nt - 1) / (8 * pl.prefix_nt));
+        split_keys(a->prefix_len, (int64_t) c->n_head_kv * pl.prefix_tiles, blocks, pl.prefix_chunk, pl.prefix_chunks);
+    }
+    const int64_t limit = (int64_t) 1 << 31;
+    if ((int64_t) a->n_seq * c->n_head_kv * pl.own_tiles * pl.own_chunks >= limit || (int64_t) c->n_head_kv * pl.prefix_tiles * pl.prefix_chunks >= limit)
+        return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
+    const size_t chunks = pl.own_chunks + pl.prefix_chunks, lines = (size_t) n_tokens * n_head;
+    if (chunks > 1) {
+        pl.part_o = lines * chunks * c->head_dim * sizeof(float);
+        pl.bytes = pl.part_o + lines * chunks * sizeof(float2);
+    }
+    return B200MOE_OK;
+}
+
+template <int D>
+int launch_join(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) ((int64_t) p.n_tokens * p.n_head));
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUDA_TRY(ctx, f32 ? cudaLaunchKernelEx(&cfg, attend_join_kernel<D, float>, p) : cudaLaunchKernelEx(&cfg, attend_join_kernel<D, __nv_bfloat16>, p));
+    return check_launch(ctx, "attention join");
+}
+
+}  // namespace
+
+namespace b200moe {
+extern template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+extern template int launch_attend<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+extern template int launch_attend<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+}  // namespace b200moe
+
+extern "C" {
+
+int b200moe_op_rope(b200moe_ctx * c, const b200moe_tensor * x, int x_type, const int32_t * pos, const b200moe_rope * r, const b200moe_tensor * dst,
+                    void * stream) {
+    ContextBase * ctx = context_base(c);
+    if (!ctx) return B200MOE_ERR_INVALID_ARG;
+    if (!elem_size(x_type)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "rows must be F32 or BF16");
+    if (!r) return fail(ctx, B200MOE_ERR_INVALID_ARG, "rope is null");
+    if (x && dst && x->ne[2] == 0 && dst->ne[2] == 0) return B200MOE_OK;
+    if (int rc = check_rows(ctx, x, x_type, "x", false)) return rc;
+    if (int rc = check_rows(ctx, dst, x_type, "dst", true)) return rc;
+    for (int i = 0; i < 3; ++i) if (x->ne[i] != dst->ne[i]) return fail(ctx, B200MOE_ERR_INVALID_ARG, "shapes differ");
+    if (!pos) return fail(ctx, B200MOE_ERR_INVALID_ARG, "pos is null");
+    if (r->n_rot < 2 || r->n_rot % 2 || r->n_rot > x->ne[0] || x->ne[0] % 2) return fail(ctx, B200MOE_ERR_INVALID_ARG, "n_rot must be even and 2 .. head_dim, head_dim even");
+    if (r->n_axes < 1 || r->n_axes > 4) return fail(ctx, B200MOE_ERR_INVALID_ARG, "1 to 4 axes");
+    if (!(r->base > 0.0) || !std::isfinite(r->base)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "base must be positive and finite");
+    const int half = r->n_rot / 2;
+    int64_t sum = 0;
+    for (int a = 0; a < r->n_axes; ++a) {
+        if (r->sections[a] < 0 || r->sections[a] > half) return fail(ctx, B200MOE_ERR_INVALID_ARG, "sections must be 0 .. n_rot / 2");
+        sum += r->sections[a];
+        // the turns that an axis gets by taking every n_axes-th pair must be there
+        if (r->interleaved && a > 0 && r->sections[a] > 0 && (int64_t) r->n_axes * (r->sections[a] - 1) + a >= half)
+            return fail(ctx, B200MOE_ERR_INVALID_ARG, "interleaved sections: axis %d has more pairs than turns", a);
+    }
+    if (sum != half) return fail(ctx, B200MOE_ERR_INVALID_ARG, "sections must sum to n_rot / 2");
+    RopeParams p = {};
+    p.x = static_cast<const char *>(x->data);
+    p.dst = static_cast<char *>(dst->data);
+    p.pos = pos;
+    p.x_head = x->nb[1]; p.x_token = x->nb[2]; p.dst_head = dst->nb[1]; p.dst_token = dst->nb[2];
+    p.n_tokens = (int) x->ne[2]; p.n_head = (int) x->ne[1]; p.head_dim = (int) x->ne[0]; p.n_rot = r->n_rot;
+    p.n_axes = r->n_axes;
+    for (int a = 0; a < 4; ++a) p.sections[a] = a < r->n_axes ? r->sections[a] : 0;
+    p.interleaved = r->interleaved != 0;
+    p.copy_rest = !(p.x == p.dst && p.x_head == p.dst_head && p.x_token == p.dst_token);
+    p.log2_step = -2.0 / r->n_rot * std::log2(r->base);
+    p.log2_turn = 2.6514961294723187;    // log2(2 pi)
+    p.sign = r->inverse ? -1.0f : 1.0f;
+    if ((int64_t) p.n_head * p.head_dim > (1 << 24)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "a token of more than 2^24 values");
+    const int vp = 16 / elem_size(x_type);
+    const bool wide = rows_aligned(x) && rows_aligned(dst) && half % vp == 0 && (p.head_dim - p.n_rot) % (2 * vp) == 0;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return x_type == B200MOE_TYPE_F32 ? launch_rope<float>(ctx, p, r->adjacent != 0, wide, st) : launch_rope<__nv_bfloat16>(ctx, p, r->adjacent != 0, wide, st);
+}
+
+int b200moe_kv_cache_bytes(const b200moe_kv_cache * cache, int64_t * value_bytes, int64_t * scale_bytes) {
+    if (!value_bytes || !scale_bytes) return B200MOE_ERR_INVALID_ARG;
+    if (int rc = check_cache_shape(nullptr, cache)) return rc;
+    const int64_t rows = cache->n_pages * cache->page_size * cache->n_head_kv;
+    *value_bytes = rows * row_bytes(cache->type, cache->head_dim);
+    *scale_bytes = rows * scale_row_bytes(cache->type, cache->head_dim);
+    return B200MOE_OK;
+}
+
+int b200moe_kv_write(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const b200moe_tensor * k, const b200moe_tensor * v, int x_type, const int32_t * slots,
+                     void * stream) {
+    return kv_move(ctx, cache, k, v, x_type, slots, true, stream);
+}
+
+int b200moe_kv_read(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const int32_t * slots, const b200moe_tensor * k, const b200moe_tensor * v, int x_type,
+                    void * stream) {
+    return kv_move(ctx, cache, k, v, x_type, slots, false, stream);
+}
+
+int b200moe_attention_workspace(b200moe_ctx * c, const b200moe_kv_cache * cache, const b200moe_attn * a, int32_t n_head, int32_t n_tokens, size_t * bytes) {
+    ContextBase * ctx = context_base(c);
+    if (!ctx) return B200MOE_ERR_INVALID_ARG;
+    if (!bytes) return fail(ctx, B200MOE_ERR_INVALID_ARG, "bytes is null");
+    if (int rc = check_attn(ctx, cache, a, n_head, n_tokens)) return rc;
+    AttnPlan bf16, f32;    // for either type of q
+    if (int rc = plan_attn(ctx, cache, a, n_head, n_tokens, false, bf16)) return rc;
+    if (int rc = plan_attn(ctx, cache, a, n_head, n_tokens, true, f32)) return rc;
+    *bytes = std::max(bf16.bytes, f32.bytes);
+    return B200MOE_OK;
+}
+
+int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b200moe_attn * a, const b200moe_tensor * q, int x_type, const b200moe_tensor * out,
+                      float * lse, void * workspace, size_t workspace_bytes, void * stream) {
+    ContextBase * ctx = context_base(c);
+    if (!ctx) return B200MOE_ERR_INVALID_ARG;
+    AttnParams p = {};
+    if (int rc = check_cache(ctx, cache, p.kv)) return rc;
+    if (!elem_size(x_type)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "q must be F32 or BF16");
+    if (!q || !out || !a) return fail(ctx, B200MOE_ERR_INVALID_ARG, "null argument");
+    if (int rc = check_attn(ctx, cache, a, q->ne[1], q->ne[2])) return rc;
+    if (q->ne[2] == 0 || a->n_seq == 0 || a->max_new == 0) return B200MOE_OK;
+    if (int rc = check_rows(ctx, q, x_type, "q", false)) return rc;
+    if (int rc = check_rows(ctx, out, x_type, "out", true)) return rc;
+    for (int i = 0; i < 3; ++i) if (q->ne[i] != out->ne[i]) return fail(ctx, B200MOE_ERR_INVALID_ARG, "q and out differ in shape");
+    if (q->ne[0] != cache->head_dim) return fail(ctx, B200MOE_ERR_INVALID_ARG, "q has another head_dim than the cache");
+    if (!a->q_start && q->ne[2] < a->n_seq) return fail(ctx, B200MOE_ERR_INVALID_ARG, "fewer tokens than sequences");
+    if (!a->kv_len || (a->max_kv_len && !a->pages) || (a->prefix_len && !a->prefix_pages)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "null lengths or pages");
+    const bool f32 = x_type == B200MOE_TYPE_F32;
+    const int n_head = (int) q->ne[1], n_tokens = (int) q->ne[2];
+    AttnPlan pl;
+    if (int rc = plan_attn(ctx, cache, a, n_head, n_tokens, f32, pl)) return rc;
+    if (pl.bytes && (!workspace || workspace_bytes < pl.bytes || ((uintptr_t) workspace & 15)))
+        return fail(ctx, B200MOE_ERR_INVALID_ARG, "the workspace must be %zu bytes and 16-byte aligned", pl.bytes);
+    p.q = static_cast<const char *>(q->data);
+    p.out = static_cast<char *>(out->data);
+    p.lse = lse;
+    p.q_head = q->nb[1]; p.q_token = q->nb[2]; p.out_head = out->nb[1]; p.out_token = out->nb[2];
+    p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / cache->n_head_kv;
+    p.n_seq = a->n_seq; p.max_new = a->q_start ? a->max_new : 1; p.max_kv_len = a->max_kv_len; p.prefix_len = a->prefix_len; p.pages_stride = a->pages_stride;
+    p.q_start = a->q_start; p.kv_len = a->kv_len; p.pages = a->pages; p.prefix_pages = a->prefix_pages;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.own_chunk = pl.own_chunk; p.own_chunks = pl.own_chunks;
+    p.prefix_chunk = pl.prefix_chunk; p.prefix_chunks = pl.prefix_chunks;
+    p.direct = pl.bytes == 0;
+    p.part_o = static_cast<float *>(workspace);
+    p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + pl.part_o);
+    p.err = ctx->d_err;
+    CUDA_TRY(ctx, cudaSetDevice(ctx->device));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto launch = [&](int nt, bool prefix, bool overlap, int blocks) {
+        if (cache->type == KV_BF16) return launch_attend<KV_BF16>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
+        if (cache->type == KV_Q8) return launch_attend<KV_Q8>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
+        return launch_attend<KV_Q4>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
+    };
+    if (pl.prefix_chunks) {
+        p.row_tiles = pl.prefix_tiles;
+        if (int rc = launch(pl.prefix_nt, true, false, pl.prefix_tiles * cache->n_head_kv * pl.prefix_chunks)) return rc;
+    }
+    p.row_tiles = pl.own_tiles;
+    if (int rc = launch(pl.own_nt, false, pl.prefix_chunks > 0, pl.own_tiles * cache->n_head_kv * pl.own_chunks * a->n_seq)) return rc;
+    if (p.direct) return B200MOE_OK;
+    if (cache->head_dim == 64) return launch_join<64>(ctx, p, f32, st);
+    if (cache->head_dim == 128) return launch_join<128>(ctx, p, f32, st);
+    return launch_join<256>(ctx, p, f32, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,236 @@
+// A cache of keys and values in pages, quantised as it is written.
+//
+// Row (page, head, place) of the keys is at ((page * n_head_kv + head) * page_size + place) * row_bytes, its scales at the same row number;
+// the values likewise.  A row's values x are held
+//   BF16  rounded to bf16;
+//   Q8    as code * d with one fp32 scale d = max|x| / 127 to the row and code = x / d rounded to the nearest whole number, halves to even;
+//   Q4    as code * d with one bf16 scale d = max|x| / 7 (rounded) to every 32 values, code in -7 .. 7.
+// d = 0 stands for a row (group) of zeros, d = NaN for one that holds an infinity or NaN: it reads back as NaN.  The codes are rounded from the
+// exact quotient: the remainder x - code * d fits fp32 without rounding (d has at most 24 bits, and the code at most 7), so one comparison
+// with half a step decides every border, and a row's codes depend on nothing but the row.
+//
+// Codes are stored with an offset that makes them unsigned (128, 8), and Q4 rows in the order in which the attention kernel's lanes hold
+// them as matrix operands (attention.cuh): in every run of up to 128 values, i.e. GB = 4 (head_dim 64: 2) groups of 32,
+//   keys    value 8c + j of group g is nibble j of 32-bit word c * GB + g;
+//   values  value 4r + j of group g is nibble j of 16-bit word r * GB + g.
+//
+// Bound by memory.  A thread holds eight values of a row (16 bytes of bf16, a whole 32-bit word of Q4 keys), the D / 8 threads of a row find
+// its largest value with shuffles, and every thread takes the key and the value row of the same place together so that both loads fly.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "rope.cuh"
+
+namespace b200moe {
+
+enum KvType : int { KV_BF16 = 0, KV_Q8 = 1, KV_Q4 = 2 };
+
+struct KvView {
+    uint8_t * k;
+    uint8_t * v;
+    void * k_scale;
+    void * v_scale;
+    int64_t n_slots;
+    int n_head;
+    int page_shift;    // log2 of the rows in a page
+};
+
+template <int TYPE, int D>
+__host__ __device__ constexpr int kv_row_bytes() { return TYPE == KV_BF16 ? 2 * D : TYPE == KV_Q8 ? D : D / 2; }
+
+// row number of a slot's head
+__device__ __forceinline__ int64_t kv_row(const KvView & c, int slot, int head) {
+    const int page = slot >> c.page_shift, at = slot & ((1 << c.page_shift) - 1);
+    return (((int64_t) page * c.n_head + head) << c.page_shift) + at;
+}
+
+struct KvRows {    // rows of a user's tensors: [token][head][head_dim], strides in bytes
+    char * k;
+    char * v;
+    int64_t k_token, k_head, v_token, v_head;
+    int aligned;    // every row starts on a 16-byte boundary
+};
+
+template <typename XT>
+__device__ __forceinline__ void load8(float (&x)[8], const char * row, int i, int aligned) {
+    const XT * p = reinterpret_cast<const XT *>(row) + 8 * i;
+    if (aligned) {
+        typedef Pack<XT, 16 / sizeof(XT)> V;
+#pragma unroll
+        for (int j = 0; j < 8; j += 16 / sizeof(XT)) {
+            const V w = *reinterpret_cast<const V *>(p + j);
+#pragma unroll
+            for (int l = 0; l < (int) (16 / sizeof(XT)); ++l) x[j + l] = to_float(w.v[l]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = to_float(p[j]);
+    }
+}
+
+template <typename XT>
+__device__ __forceinline__ void store8(const float (&x)[8], char * row, int i, int aligned) {
+    XT * p = reinterpret_cast<XT *>(row) + 8 * i;
+    if (aligned) {
+        typedef Pack<XT, 16 / sizeof(XT)> V;
+#pragma unroll
+        for (int j = 0; j < 8; j += 16 / sizeof(XT)) {
+            V w;
+#pragma unroll
+            for (int l = 0; l < (int) (16 / sizeof(XT)); ++l) w.v[l] = from_float<XT>(x[j + l]);
+            *reinterpret_cast<V *>(p + j) = w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = from_float<XT>(x[j]);
+    }
+}
+
+// round-half-even(x / d), at most `top` in size; inv about 1 / d
+__device__ __forceinline__ int kv_code(float x, float d, float inv, int top) {
+    const float q = rintf(x * inv);
+    const float r = __fmaf_rn(-q, d, x);             // exact: see above
+    const float over = 2.0f * fabsf(r);
+    int code = (int) q;
+    if (over > d || (over == d && (code & 1))) code += r > 0.0f ? 1 : -1;
+    return max(-top, min(top, code));
+}
+
+// the largest |x| of a group as its bits, which order infinities and NaN behind every number; GROUP threads
+template <int GROUP>
+__device__ __forceinline__ uint32_t group_amax(const float (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = GROUP / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+template <int TYPE, int D, bool VALUES>
+__device__ __forceinline__ void kv_store_row(const float (&x)[8], uint8_t * rows, void * scales, int64_t row, int i, bool on) {
+    uint8_t * at = rows + row * kv_row_bytes<TYPE, D>();
+    if (TYPE == KV_BF16) {
+        if (on) store8<__nv_bfloat16>(x, reinterpret_cast<char *>(at), i, 1);
+        return;
+    }
+    constexpr int TOP = TYPE == KV_Q8 ? 127 : 7;
+    const uint32_t bits = group_amax<TYPE == KV_Q8 ? D / 8 : 4>(x);
+    float d = bits < 0x7f800000u ? __fdiv_rn(__uint_as_float(bits), (float) TOP) : __uint_as_float(0x7fffffffu);
+    if (TYPE == KV_Q4) d = __bfloat162float(__float2bfloat16_rn(d));
+    int code[8];
+    // below 2^-120 the reciprocal, or a product with it, may leave the normal range: divide
+    const float inv = d >= 0x1p-120f ? __frcp_rn(d) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        code[j] = 0;
+        if (inv > 0.0f) code[j] = kv_code(x[j], d, inv, TOP);
+        else if (d > 0.0f) code[j] = max(-TOP, min(TOP, (int) rint((double) x[j] / (double) d)));
+    }
+    if (!on) return;
+    if (TYPE == KV_Q8) {
+        uint32_t w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            w[j] = (uint32_t) (code[4 * j] + 128) | (uint32_t) (code[4 * j + 1] + 128) << 8 | (uint32_t) (code[4 * j + 2] + 128) << 16 |
+                   (uint32_t) (code[4 * j + 3] + 128) << 24;
+        *reinterpret_cast<uint2 *>(at + 8 * i) = make_uint2(w[0], w[1]);
+        if (i == 0) static_cast<float *>(scales)[row] = d;
+    } else {
+        constexpr int GB = D >= 128 ? 4 : 2;    // groups of 32 in a run
+        const int g = i / 4, c = i % 4, run = g / GB, gr = g % GB;
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w |= (uint32_t) (code[j] + 8) << (4 * j);
+        uint8_t * p = at + run * 16 * GB;
+        if (VALUES) {
+            *reinterpret_cast<uint16_t *>(p + 2 * ((2 * c) * GB + gr)) = (uint16_t) w;
+            *reinterpret_cast<uint16_t *>(p + 2 * ((2 * c + 1) * GB + gr)) = (uint16_t) (w >> 16);
+        } else {
+            *reinterpret_cast<uint32_t *>(p + 4 * (c * GB + gr)) = w;
+        }
+        if (c == 0) static_cast<__nv_bfloat16 *>(scales)[row * (D / 32) + g] = __float2bfloat16_rn(d);
+    }
+}
+
+template <int TYPE, int D, bool VALUES>
+__device__ __forceinline__ void kv_load_row(float (&x)[8], const uint8_t * rows, const void * scales, int64_t row, int i) {
+    const uint8_t * at = rows + row * kv_row_bytes<TYPE, D>();
+    if (TYPE == KV_BF16) {
+        load8<__nv_bfloat16>(x, reinterpret_cast<const char *>(at), i, 1);
+    } else if (TYPE == KV_Q8) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(at + 8 * i);
+        const float d = static_cast<const float *>(scales)[row];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = d * (float) ((int) (((j < 4 ? w.x : w.y) >> (8 * (j % 4))) & 255u) - 128);
+    } else {
+        constexpr int GB = D >= 128 ? 4 : 2;
+        const int g = i / 4, c = i % 4, run = g / GB, gr = g % GB;
+        const uint8_t * p = at + run * 16 * GB;
+        uint32_t w;
+        if (VALUES)
+            w = *reinterpret_cast<const uint16_t *>(p + 2 * ((2 * c) * GB + gr)) |
+                (uint32_t) *reinterpret_cast<const uint16_t *>(p + 2 * ((2 * c + 1) * GB + gr)) << 16;
+        else
+            w = *reinterpret_cast<const uint32_t *>(p + 4 * (c * GB + gr));
+        const float d = __bfloat162float(static_cast<const __nv_bfloat16 *>(scales)[row * (D / 32) + g]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = d * (float) ((int) ((w >> (4 * j)) & 15u) - 8);
+    }
+}
+
+constexpr int KV_THREADS = 256;
+
+// D / 8 threads to a (token, head); slots below zero are passed over
+template <int TYPE, int D, typename XT>
+__global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const KvView c, const KvRows x, const int32_t * slots, int64_t n_rows, int * err) {
+    constexpr int ROWS = KV_THREADS / (D / 8);
+    const int i = threadIdx.x % (D / 8);
+    for (int64_t r0 = (int64_t) blockIdx.x * ROWS; r0 < n_rows; r0 += (int64_t) gridDim.x * ROWS) {
+        const int64_t r = r0 + threadIdx.x / (D / 8);
+        const bool there = r < n_rows;
+        const int64_t t = there ? r / c.n_head : 0;
+        const int h = there ? (int) (r - t * c.n_head) : 0;
+        const int slot = there ? slots[t] : -1;
+        if (slot >= c.n_slots && i == 0) report_error(err, DEV_ERR_BAD_SLOT);
+        const bool on = slot >= 0 && slot < c.n_slots;
+        float k[8], v[8];
+        if (on) {
+            load8<XT>(k, x.k + t * x.k_token + h * x.k_head, i, x.aligned);
+            load8<XT>(v, x.v + t * x.v_token + h * x.v_head, i, x.aligned);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.0f;
+        }
+        const int64_t row = on ? kv_row(c, slot, h) : 0;
+        kv_store_row<TYPE, D, false>(k, c.k, c.k_scale, row, i, on);
+        kv_store_row<TYPE, D, true>(v, c.v, c.v_scale, row, i, on);
+    }
+}
+
+// the other way; rows of slots below zero are zeros
+template <int TYPE, int D, typename XT>
+__global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const KvView c, const KvRows x, const int32_t * slots, int64_t n_rows, int * err) {
+    constexpr int ROWS = KV_THREADS / (D / 8);
+    const int i = threadIdx.x % (D / 8);
+    for (int64_t r = (int64_t) blockIdx.x * ROWS + threadIdx.x / (D / 8); r < n_rows; r += (int64_t) gridDim.x * ROWS) {
+        const int64_t t = r / c.n_head;
+        const int h = (int) (r - t * c.n_head);
+        const int slot = slots[t];
+        if (slot >= c.n_slots && i == 0) report_error(err, DEV_ERR_BAD_SLOT);
+        float k[8], v[8];
+        if (slot >= 0 && slot < c.n_slots) {
+            const int64_t row = kv_row(c, slot, h);
+            kv_load_row<TYPE, D, false>(k, c.k, c.k_scale, row, i);
+            kv_load_row<TYPE, D, true>(v, c.v, c.v_scale, row, i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = v[j] = 0.0f;
+        }
+        store8<XT>(k, x.k + t * x.k_token + h * x.k_head, i, x.aligned);
+        store8<XT>(v, x.v + t * x.v_token + h * x.v_head, i, x.aligned);
+    }
+}
+
+}  // namespace b200moe

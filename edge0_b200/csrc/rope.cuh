@@ -1,0 +1,126 @@
+// Rotary positions with one to four axes.
+//
+// Pair i of the n_rot / 2 pairs of a head belongs to axis a(i) and turns by w = pos[a(i)][t] * base^(-2i / n_rot):
+//     (x0, x1) -> (x0 cos w - x1 sin w, x0 sin w + x1 cos w),
+// with pairs (i, i + n_rot / 2) or (2i, 2i + 1).  The inverse turns by -w, which is also the gradient's way back (the matrix is orthogonal).
+//
+// Angles: positions far into a context times a frequency near 1 lose all of fp32's bits, so the turn is worked out in whole revolutions in
+// double (pos * 2^(i c - log2 2 pi), the whole part taken off) and only the rest, below half a revolution, goes to the fp32 sine and cosine.
+// The four products of a pair are fp32, rounded once to the output's type.
+//
+// Bound by memory: every value is read and written once.  A block takes a few tokens, works out their pairs' sines and cosines once into
+// shared memory (a table entry serves every head of the token) and then runs over the heads with 16-byte loads and stores; rows or strides
+// that are not multiples of 16 bytes go pair by pair.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace b200moe {
+
+struct RopeParams {
+    const char * x;
+    char * dst;
+    const int32_t * pos;                             // [n_axes][n_tokens]
+    int64_t x_head, x_token, dst_head, dst_token;    // strides in bytes
+    int n_tokens, n_head, head_dim, n_rot;
+    int n_axes, sections[4];
+    int interleaved;
+    int copy_rest;        // the values behind n_rot are copied (not when dst is x)
+    double log2_step;     // -2 / n_rot * log2(base)
+    double log2_turn;     // log2(2 pi)
+    float sign;           // -1: inverse
+};
+
+__device__ __forceinline__ int rope_axis(const RopeParams & p, int pair) {
+    if (p.interleaved) {
+        const int a = pair % p.n_axes;
+        return pair < p.n_axes * p.sections[a] ? a : 0;
+    }
+    int a = 0, end = p.sections[0];
+    while (a + 1 < p.n_axes && pair >= end) end += p.sections[++a];
+    return a;
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_ITEMS = 4;    // items of a thread whose loads are in flight together
+
+// VP pairs to an item: 16 bytes of either half of a pair, or 1 where that is not aligned
+template <typename T, int VP, bool ADJACENT>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeParams p, int tokens_per_block) {
+    extern __shared__ float2 turn[];    // [tokens_per_block][n_rot / 2]
+    typedef Pack<T, VP> V;
+    const int half = p.n_rot / 2;
+    const int t0 = blockIdx.x * tokens_per_block, nt = min(tokens_per_block, p.n_tokens - t0);
+    for (int e = threadIdx.x; e < nt * half; e += ROPE_THREADS) {
+        const int t = e / half, i = e - t * half;
+        const double pos = (double) p.pos[(int64_t) rope_axis(p, i) * p.n_tokens + t0 + t];
+        double r = pos * exp2((double) i * p.log2_step - p.log2_turn);
+        r -= rint(r);
+        float s, c;
+        sincospif(2.0f * (float) r, &s, &c);
+        turn[e] = make_float2(c, p.sign * s);
+    }
+    __syncthreads();
+
+    const int turned = half / VP, rest = p.copy_rest ? (p.head_dim - p.n_rot) / (2 * VP) : 0;
+    const int per_head = turned + rest, per_token = per_head * p.n_head;
+    for (int base = threadIdx.x; base < nt * per_token; base += ROPE_THREADS * ROPE_ITEMS) {
+        V a[ROPE_ITEMS], b[ROPE_ITEMS];
+#pragma unroll
+        for (int u = 0; u < ROPE_ITEMS; ++u) {
+            const int e = base + u * ROPE_THREADS;
+            if (e >= nt * per_token) break;
+            const int t = e / per_token, q = e - t * per_token, h = q / per_head, i = (q - h * per_head) * VP;
+            const T * row = reinterpret_cast<const T *>(p.x + (int64_t) (t0 + t) * p.x_token + (int64_t) h * p.x_head);
+            // behind the turned pairs: 2 VP values at n_rot + 2 (i - half), as for pairs of neighbours
+            const bool flat = ADJACENT || i >= half;
+            a[u] = *reinterpret_cast<const V *>(row + (flat ? 2 * i : i));
+            b[u] = *reinterpret_cast<const V *>(row + (flat ? 2 * i + VP : i + half));
+        }
+#pragma unroll
+        for (int u = 0; u < ROPE_ITEMS; ++u) {
+            const int e = base + u * ROPE_THREADS;
+            if (e >= nt * per_token) break;
+            const int t = e / per_token, q = e - t * per_token, h = q / per_head, i = (q - h * per_head) * VP;
+            T * row = reinterpret_cast<T *>(p.dst + (int64_t) (t0 + t) * p.dst_token + (int64_t) h * p.dst_head);
+            const bool flat = ADJACENT || i >= half;
+            V c = a[u], d = b[u];
+            if (i < half) {
+#pragma unroll
+                for (int j = 0; j < VP; ++j) {
+                    const float2 w = turn[t * half + i + j];
+                    if (ADJACENT) {    // pair j is values 2j, 2j + 1 of the 2 VP
+                        const float x0 = to_float(2 * j < VP ? a[u].v[(2 * j) % VP] : b[u].v[(2 * j) % VP]);
+                        const float x1 = to_float(2 * j + 1 < VP ? a[u].v[(2 * j + 1) % VP] : b[u].v[(2 * j + 1) % VP]);
+                        const T y0 = from_float<T>(x0 * w.x - x1 * w.y), y1 = from_float<T>(x0 * w.y + x1 * w.x);
+                        if (2 * j < VP) c.v[(2 * j) % VP] = y0;
+                        else d.v[(2 * j) % VP] = y0;
+                        if (2 * j + 1 < VP) c.v[(2 * j + 1) % VP] = y1;
+                        else d.v[(2 * j + 1) % VP] = y1;
+                    } else {
+                        const float x0 = to_float(a[u].v[j]), x1 = to_float(b[u].v[j]);
+                        c.v[j] = from_float<T>(x0 * w.x - x1 * w.y);
+                        d.v[j] = from_float<T>(x0 * w.y + x1 * w.x);
+                    }
+                }
+            }
+            *reinterpret_cast<V *>(row + (flat ? 2 * i : i)) = c;
+            *reinterpret_cast<V *>(row + (flat ? 2 * i + VP : i + half)) = d;
+        }
+    }
+}
+
+}  // namespace b200moe

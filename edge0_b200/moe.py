@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .capi import TYPE_BF16, TYPE_F32, TYPE_NVFP4, TYPE_Q3_K, B200MoeError, Layer, Observe
+from .capi import TYPE_BF16, TYPE_F32, TYPE_NVFP4, TYPE_Q3_K, B200MoeError, Layer, Observe, Rope, Tensor
 
 TYPE_BY_NAME = {"q3_k": TYPE_Q3_K, "nvfp4": TYPE_NVFP4}
 
@@ -59,6 +59,27 @@ def _x_type(x: torch.Tensor) -> int:
     if x.dtype == torch.bfloat16:
         return TYPE_BF16
     raise TypeError("activations must be float32 or bfloat16")
+
+
+def rows_view(t: torch.Tensor, what: str) -> Tensor:
+    """b200moe_tensor of rows [T, heads, head_dim] (any strides between tokens and heads; the values of a row side by side)."""
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] != 1):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous rows, not {tuple(t.shape)} with strides {t.stride()}")
+    n, h, d = t.shape
+    es = t.element_size()
+    v = Tensor(t.data_ptr())
+    v.ne[:] = (d, h, n, 1)
+    v.nb[:] = (es, t.stride(1) * es, t.stride(0) * es, 0)
+    return v
+
+
+def int32_on(t: torch.Tensor, device: torch.device, what: str, shape=None) -> C.c_void_p:
+    """Pointer of a contiguous int32 tensor on `device` (of `shape`, where given)."""
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    return C.c_void_p(t.data_ptr())
 
 
 def unpack_expert_blobs_nvfp4(blobs: np.ndarray, n_embd: int, n_ff: int, device=None):
@@ -231,6 +252,26 @@ class Context:
         dst = torch.empty((idx.shape[0], src.shape[1]), dtype=torch.float32, device=src.device)
         self.check(self.lib.b200moe_gather_rows(self.handle, _ptr(src), src.shape[0], _ptr(idx), _ptr(dst), idx.shape[0], src.shape[1], self._stream()))
         return dst
+
+    def rope(self, x: torch.Tensor, pos: torch.Tensor, *, base: float = 1e6, n_rot: Optional[int] = None, sections=None, interleaved: bool = False,
+             adjacent: bool = False, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Rotary positions (b200moe_op_rope): x [T, heads, head_dim] float32 or bfloat16, any strides between tokens and heads; pos int32 [T], or
+        [axes, T] with `sections` pairs to each axis.  inverse: the way back, also for gradients.  out may be x itself."""
+        device = torch.device("cuda", self.device)
+        if x.device != device:
+            raise ValueError(f"x must be on {device}")
+        T, _, d = x.shape
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=device)
+        elif out.dtype != x.dtype or out.device != device or out.shape != x.shape:
+            raise ValueError("out must be like x")
+        r = Rope(n_rot=d if n_rot is None else n_rot, interleaved=interleaved, adjacent=adjacent, inverse=inverse, base=base)
+        sections = [r.n_rot // 2] if sections is None else list(sections)
+        r.n_axes = len(sections)
+        r.sections[:len(sections[:4])] = sections[:4]
+        p = int32_on(pos, device, "pos", (T,) if len(sections) == 1 and pos.dim() == 1 else (len(sections), T))
+        self.check(self.lib.b200moe_op_rope(self.handle, C.byref(rows_view(x, "x")), _x_type(x), p, C.byref(r), C.byref(rows_view(out, "out")), self._stream()))
+        return out
 
     # ---- expert-parallel exchange (b200moe_ep_*): outputs may be passed in so a step allocates nothing
     def ep_pack(self, rows: torch.Tensor, ids: torch.Tensor, n_ranks: int, experts_per_rank: int, capacity: int,

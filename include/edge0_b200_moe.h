@@ -323,6 +323,95 @@ B200MOE_API int b200moe_op_argsort_desc(b200moe_ctx * ctx, const b200moe_tensor 
 B200MOE_API int b200moe_op_mul_mat_f32(b200moe_ctx * ctx, const float * w, int64_t ne00, int64_t ne01, const float * x, int64_t n_tokens, float * dst,
                                        void * stream);
 
+/* ---- the attention half of a decoder layer, which stands in front of the MoE FFN: rotary positions, a cache of keys and values that is
+ * quantised as it is written, and attention over it for a batch of sequences that may share a prefix (reference: Builder::attention,
+ * edge0-infer/src/models/edge0_35b/forward.cpp:174-214: ggml_rope, the session's cache, ggml_flash_attn_ext).  Activations are F32 or BF16
+ * tensors described as ggml does, ne = [head_dim, heads, tokens, 1], elements of a row side by side (nb[0] = their size), any strides
+ * between heads and tokens: a slice of a fused projection goes in as it is.  Rows whose addresses are multiples of 16 bytes are fastest. */
+
+/* Rotary positions with one to four axes (text: one; images and video: time, height, width).  Pair i of a head's n_rot / 2 pairs turns by
+ * pos[axis(i)][token] * base^(-2i / n_rot); the values behind n_rot are copied.  Pairs are (i, i + n_rot / 2), with `adjacent` (2i, 2i + 1).
+ * sections[a] pairs belong to axis a, one section behind the other; with `interleaved` the axes take turns: pair i belongs to axis i % n_axes
+ * while i < n_axes * sections[i % n_axes], to axis 0 else.  `inverse` turns the other way, which is also how a gradient goes back.
+ * Angles are worked out in double before the whole turns are taken off, so far positions lose nothing.  pos: I32 [tokens, n_axes], any values.
+ * dst may be x itself (same strides) and must not overlap it in any other way. */
+typedef struct b200moe_rope {
+    int32_t n_rot;          /* even, 2 .. head_dim */
+    int32_t n_axes;         /* 1 .. 4 */
+    int32_t sections[4];    /* sum n_rot / 2 */
+    int32_t interleaved;
+    int32_t adjacent;
+    int32_t inverse;
+    int32_t reserved_;
+    double  base;
+} b200moe_rope;
+B200MOE_API int b200moe_op_rope(b200moe_ctx * ctx, const b200moe_tensor * x, int x_type, const int32_t * pos, const b200moe_rope * rope,
+                                const b200moe_tensor * dst, void * stream);
+
+/* A cache of n_pages pages of page_size positions for the n_head_kv heads of one layer.  The four arrays are the caller's
+ * (b200moe_kv_cache_bytes says how large; 16-byte aligned); what is in them is written by b200moe_kv_write and read by b200moe_kv_read and
+ * b200moe_attention only, but pages may be copied as they are: page i is the i-th n_pages-th part of each array.
+ * A slot is a position's number in the cache, page * page_size + place in the page.
+ *   B200MOE_KV_BF16  rows rounded to bf16; no scales (k_scale, v_scale NULL)
+ *   B200MOE_KV_Q8    8 bits a value and one F32 scale d = max|x| / 127 a row: x is held as d * round(x / d)
+ *   B200MOE_KV_Q4    4 bits a value (-7 .. 7) and one bf16 scale max|x| / 7 to every 32 values
+ * Halves round to even, the quotient is exact (unlike ggml's Q8_0, which multiplies by a rounded reciprocal and scales every 32 values): a held value
+ * is at most half a step from x (Q4: the scale's rounding to bf16 comes on top for a group's largest value, 2^-9 of it).  A row (Q4: group)
+ * with an infinity or NaN reads back as NaN.  head_dim 64, 128 or 256; page_size 16, 32, 64, 128 or 256; fewer than 2^31 slots. */
+enum b200moe_kv_type { B200MOE_KV_BF16 = 0, B200MOE_KV_Q8 = 1, B200MOE_KV_Q4 = 2 };
+typedef struct b200moe_kv_cache {
+    int32_t type;
+    int32_t n_head_kv;
+    int32_t head_dim;
+    int32_t page_size;
+    int64_t n_pages;
+    void *  k;
+    void *  v;
+    void *  k_scale;
+    void *  v_scale;
+} b200moe_kv_cache;
+/* bytes of k (and of v), and of k_scale (and of v_scale); the pointers of `cache` are not looked at */
+B200MOE_API int b200moe_kv_cache_bytes(const b200moe_kv_cache * cache, int64_t * value_bytes, int64_t * scale_bytes);
+/* The rows of tokens 0 .. T-1 of k and v (ne = [head_dim, n_head_kv, T, 1]) go to slots[0 .. T-1] (device).  A slot below zero is passed
+ * over (padding); one that the cache does not have is passed over and reported by b200moe_synchronize.  Slots must differ: a slot
+ * that is named twice holds parts of either row afterwards. */
+B200MOE_API int b200moe_kv_write(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const b200moe_tensor * k, const b200moe_tensor * v, int x_type,
+                                 const int32_t * slots, void * stream);
+/* The other way: the values that slots[0 .. T-1] hold, in F32 or BF16 (x_type); a slot below zero, or not of the cache (reported), gives zeros. */
+B200MOE_API int b200moe_kv_read(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const int32_t * slots, const b200moe_tensor * k,
+                                const b200moe_tensor * v, int x_type, void * stream);
+
+/* Attention of n_seq sequences over the cache.  Sequence b has the new tokens q_start[b] .. q_start[b + 1] - 1 of q and kv_len[b] positions of its
+ * own in the cache, the new tokens' (written before) the last of them; its position i is place i % page_size of page pages[b][i / page_size].
+ * In front of every sequence's own positions stand the prefix_len positions of prefix_pages, which are read once for the whole batch.  A token
+ * sees the prefix and its sequence's positions up to its own:  out = sum_j softmax_j(scale * q . k_j) v_j  over those, zeros where there are none.
+ * Query head h reads key/value head h / (n_head / n_head_kv).  Lengths and tables are on the device, so that a captured graph may be
+ * replayed with others; the host's max_new, max_kv_len bound what the lengths may be in any replay.  Rows of q and out behind
+ * q_start[n_seq] belong to nobody and are left as they are, as are those of a sequence whose lengths break the bounds, which b200moe_synchronize
+ * reports like a page that the cache does not have (its positions count as unseen).  What lies in the cache behind a sequence's length, or
+ * a token's reach, has no influence, whatever it is; an infinity or NaN within reach makes outputs infinite or NaN.
+ * lse (or NULL): F32 [n_head, tokens], the natural logarithm of the sum of exp(scale * q . k_j), -inf where there are no positions.
+ * BF16 queries: products of the held values in full, weights rounded to 2^-12 or less of each; F32: everything to fp32's accuracy. */
+typedef struct b200moe_attn {
+    int32_t n_seq;
+    int32_t max_new;                 /* most new tokens of a sequence */
+    int32_t max_kv_len;              /* most positions of a sequence, at most pages_stride * page_size */
+    int32_t prefix_len;              /* 0: no prefix */
+    int32_t pages_stride;            /* entries of `pages` from one sequence to the next */
+    float   scale;
+    const int32_t * q_start;         /* [n_seq + 1], ascending from 0; NULL: one new token a sequence, n_seq tokens */
+    const int32_t * kv_len;          /* [n_seq] */
+    const int32_t * pages;           /* [n_seq][pages_stride] */
+    const int32_t * prefix_pages;    /* [ceil(prefix_len / page_size)] */
+} b200moe_attn;
+/* Bytes of the workspace that a call needs for n_tokens rows of q (0 where none is needed); it depends on the sizes only, the pointers of `attn` are not looked at */
+B200MOE_API int b200moe_attention_workspace(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const b200moe_attn * attn, int32_t n_head,
+                                            int32_t n_tokens, size_t * bytes);
+/* q, out: ne = [head_dim, n_head, tokens, 1] of x_type (F32 or BF16).  workspace: device memory of the caller's, 16-byte aligned, which
+ * calls that may run at the same time must not share; nothing in it is kept from one call to the next. */
+B200MOE_API int b200moe_attention(b200moe_ctx * ctx, const b200moe_kv_cache * cache, const b200moe_attn * attn, const b200moe_tensor * q, int x_type,
+                                  const b200moe_tensor * out, float * lse, void * workspace, size_t workspace_bytes, void * stream);
+
 /* ---- probe of the block-scaled FP4 tensor-core instruction (tcgen05.mma kind::mxf4nvf4, UE4M3 scale per 16 values; the reference's only
  * Blackwell kernel is the warp-level form of it, ggml-cuda/mma.cuh:1186-1214).  Not part of the layer: it pins the operand formats
  * the FP4 engine relies on and measures the denominator of "% of FP4 peak".  Both allocate and free their own device memory.

@@ -1,0 +1,18 @@
+"""Argument checks of rotary positions, the cache and attention over it (tests/decoder_ops_refusals.cpp): every refused call is refused
+before a launch, on a context whose device does not exist."""
+import os
+import subprocess
+
+from edge0_b200 import build, capi
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def test_entry_points_refuse_what_the_header_forbids(tmp_path):
+    capi.load()
+    exe = str(tmp_path / "refusals")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(build.nvcc())))
+    subprocess.check_call(["g++", "-std=c++17", "-O0", "-I", os.path.join(cuda, "include"), "-o", exe, os.path.join(HERE, "decoder_ops_refusals.cpp"), capi.LIB_PATH,
+                           "-Wl,-rpath," + os.path.dirname(capi.LIB_PATH), "-L" + os.path.join(cuda, "lib64"), "-lcudart"])
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120, env=dict(os.environ, LD_LIBRARY_PATH=os.path.join(cuda, "lib64")))
+    assert r.returncode == 0, r.stdout + r.stderr
