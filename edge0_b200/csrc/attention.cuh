@@ -45,6 +45,8 @@ struct AttnParams {
     float scale_log2;                                // scale * log2(e)
     int own_chunk, own_chunks;                       // keys to a chunk, most chunks of a sequence (0: there are no own keys)
     int prefix_chunk, prefix_chunks;
+    int own_prefix;                                  // positions of the prefix that the own keys' kernel walks in front of them (attention_tc.cuh)
+    int q_aligned, out_aligned;                      // rows start on 16-byte boundaries
     int row_tiles;                                   // of the launch: tiles of rows per sequence (own) or of the whole batch (prefix)
     int direct;                                      // one chunk in all: the block writes the result itself
     float * part_o;                                  // [n_tokens * n_head][chunks][D]
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
     }
     int first, n_new, len;
     if (seq >= p.n_seq || !attn_sequence(p, seq, first, n_new, len, false) || token < first || token >= first + n_new) return;    // a row that belongs to nobody
-    const int reach = max(0, len - n_new + (token - first) + 1);
+    const int reach = p.own_prefix + max(0, len - n_new + (token - first) + 1);
     const int own = p.own_chunks ? (reach + p.own_chunk - 1) / p.own_chunk : 0;
     const int n = p.prefix_chunks + own, chunks = p.prefix_chunks + p.own_chunks;
     const float2 * ml = p.part_ml + line * chunks;
@@ -771,6 +773,10 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
 // (at most attend_tiles()); overlap: the own keys' kernel starts beside the prefix's.
 template <int TYPE>
 int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st);
+
+// The same for bf16 queries and tiles of 128 rows (attention_tc.cuh), a launch of its own in every case.
+template <int TYPE>
+int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, int blocks, cudaStream_t st);
 
 // most rows to a tile / 8: what leaves the outputs and the loads in registers
 inline int attend_tiles(int head_dim, bool f32) { return f32 || head_dim == 256 ? 2 : 4; }

@@ -1,22 +1,30 @@
 // Launches of the attention kernels for one type of cache; included by that type's translation unit alone.
 #pragma once
 #include "attention.cuh"
+#include "attention_tc.cuh"
 
 namespace b200moe {
 
 constexpr int ATTN_MAX_DEVICES = 64;
 
+// raises a kernel's limit of dynamic shared memory, an attribute of the (function, device) pair, once
+template <typename Kern>
+int raise_shared_limit(ContextBase * ctx, Kern kern, size_t smem, bool (&done)[ATTN_MAX_DEVICES]) {
+    if (ctx->device < 0 || ctx->device >= ATTN_MAX_DEVICES) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "device ordinal %d out of range", ctx->device);
+    if (!done[ctx->device]) {
+        CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
+        done[ctx->device] = true;
+    }
+    return B200MOE_OK;
+}
+
 template <int TYPE, int D, typename XT, int NT, bool PREFIX>
 int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int blocks, cudaStream_t st) {
     auto kern = attend_kernel<TYPE, D, XT, NT, PREFIX>;
     constexpr size_t smem = AttnShape<TYPE, D, XT, NT>::SMEM;
-    if (smem > 48 * 1024) {    // an attribute of the (function, device) pair
+    if (smem > 48 * 1024) {
         static bool done[ATTN_MAX_DEVICES] = {};
-        if (ctx->device >= ATTN_MAX_DEVICES) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "device ordinal %d out of range", ctx->device);
-        if (!done[ctx->device]) {
-            CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem));
-            done[ctx->device] = true;
-        }
+        if (int rc = raise_shared_limit(ctx, kern, smem, done)) return rc;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) blocks);
@@ -52,6 +60,23 @@ int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f3
     if (head_dim == 64) return launch_attend_d<TYPE, 64>(ctx, p, f32, nt, prefix, overlap, blocks, st);
     if (head_dim == 128) return launch_attend_d<TYPE, 128>(ctx, p, f32, nt, prefix, overlap, blocks, st);
     return launch_attend_d<TYPE, 256>(ctx, p, f32, nt, prefix, overlap, blocks, st);
+}
+
+template <int TYPE, int D, bool PREFIX>
+int launch_attend_tc_t(ContextBase * ctx, const AttnParams & p, int blocks, cudaStream_t st) {
+    auto kern = attend_tc_kernel<TYPE, D, PREFIX>;
+    constexpr size_t smem = TcShape<TYPE, D>::SMEM;
+    static bool done[ATTN_MAX_DEVICES] = {};
+    if (int rc = raise_shared_limit(ctx, kern, smem, done)) return rc;
+    kern<<<(unsigned) blocks, TC_THREADS, smem, st>>>(p);
+    return check_launch(ctx, "attention, 128 rows to a tile");
+}
+
+template <int TYPE>
+int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, int blocks, cudaStream_t st) {
+    if (head_dim == 64) return prefix ? launch_attend_tc_t<TYPE, 64, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 64, false>(ctx, p, blocks, st);
+    if (head_dim == 128) return prefix ? launch_attend_tc_t<TYPE, 128, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 128, false>(ctx, p, blocks, st);
+    return prefix ? launch_attend_tc_t<TYPE, 256, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 256, false>(ctx, p, blocks, st);
 }
 
 }  // namespace b200moe

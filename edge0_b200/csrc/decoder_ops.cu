@@ -128,19 +128,22 @@ int kv_move(b200moe_ctx * c, const b200moe_kv_cache * cache, const b200moe_tenso
 
 // ---- attention
 struct AttnPlan {
-    int own_nt, own_tiles, own_chunk, own_chunks;
+    int own_nt, own_tiles, own_chunk, own_chunks;    // nt: rows to a tile / 8
     int prefix_nt, prefix_tiles, prefix_chunk, prefix_chunks;
+    int own_prefix;
     size_t part_o, bytes;
 };
 
+// From so many rows to a key/value head the kernels with 128 rows to a tile run (bf16 queries).
+constexpr int ATTN_TC_ROWS = 64;
+constexpr int TC_TILE = 16;    // nt of the kernels with 128 rows to a tile
+
 int tile_units(int64_t rows, int most) { return rows <= 8 ? 1 : rows <= 16 ? 2 : most; }
 
-// keys to a chunk, so that `base` blocks of whole length become about `blocks`
-void split_keys(int64_t len, int64_t base, int64_t blocks, int & chunk, int & chunks) {
-    constexpr int UNIT = 32 * ATTN_WARPS;    // a pass of every warp of a block
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((len + UNIT - 1) / UNIT, blocks / std::max<int64_t>(base, 1)));
-    chunk = (int) (((len + n - 1) / n + UNIT - 1) / UNIT * UNIT);
-    chunk = std::max(chunk, UNIT);
+// keys to a chunk, a multiple of `unit`, so that `base` blocks of whole length become about `blocks`
+void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int & chunk, int & chunks) {
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((len + unit - 1) / unit, blocks / std::max<int64_t>(base, 1)));
+    chunk = (int) std::max<int64_t>(unit, ((len + n - 1) / n + unit - 1) / unit * unit);
     chunks = (int) ((len + chunk - 1) / chunk);
 }
 
@@ -152,25 +155,30 @@ int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn
     if (n_head % c->n_head_kv) return fail(ctx, B200MOE_ERR_INVALID_ARG, "n_head must be a multiple of n_head_kv");
     if (!std::isfinite(a->scale)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "scale must be finite");
     if ((int64_t) a->pages_stride * c->page_size < a->max_kv_len) return fail(ctx, B200MOE_ERR_INVALID_ARG, "max_kv_len needs more pages than a sequence's table has");
-    if (a->max_kv_len > INT32_MAX / 2 || a->prefix_len > INT32_MAX / 2) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "at most 2^30 positions");
+    if (a->max_kv_len > INT32_MAX / 4 || a->prefix_len > INT32_MAX / 4) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "at most 2^29 positions");
     if (n_tokens * n_head >= ((int64_t) 1 << 31) || (int64_t) a->max_new * n_head >= ((int64_t) 1 << 31)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
     return B200MOE_OK;
 }
 
 int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int n_head, int n_tokens, bool f32, AttnPlan & pl) {
     const int group = n_head / c->n_head_kv, most = attend_tiles(c->head_dim, f32);
+    const int pass = 32 * ATTN_WARPS, tc_pass = c->head_dim == 256 ? 64 : 128;
     const int64_t blocks = (int64_t) ctx->sm_count * 6;
     pl = AttnPlan{};
-    const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group;
-    pl.own_nt = tile_units(own_rows, most);
+    const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
+    const bool own_tc = !f32 && own_rows >= ATTN_TC_ROWS, prefix_tc = !f32 && rows >= ATTN_TC_ROWS;
+    // sequences that fill tiles of their own walk the prefix themselves: the products take the same time, and nothing is left to join
+    if (a->prefix_len && own_tc && own_rows >= 128) pl.own_prefix = a->prefix_len;
+    pl.own_nt = own_tc ? TC_TILE : tile_units(own_rows, most);
     pl.own_tiles = (int) ((own_rows + 8 * pl.own_nt - 1) / (8 * pl.own_nt));
-    split_keys(a->max_kv_len, (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, blocks, pl.own_chunk, pl.own_chunks);
+    split_keys((int64_t) a->max_kv_len + pl.own_prefix, (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, own_tc ? ctx->sm_count : blocks,
+               own_tc ? tc_pass : pass, pl.own_chunk, pl.own_chunks);
     pl.own_chunks = std::max(pl.own_chunks, 1);
-    if (a->prefix_len) {
-        const int64_t rows = (int64_t) n_tokens * group;
-        pl.prefix_nt = tile_units(rows, most);
+    if (a->prefix_len && !pl.own_prefix) {
+        pl.prefix_nt = prefix_tc ? TC_TILE : tile_units(rows, most);
         pl.prefix_tiles = (int) ((rows + 8 * pl.prefix_nt - 1) / (8 * pl.prefix_nt));
-        split_keys(a->prefix_len, (int64_t) c->n_head_kv * pl.prefix_tiles, blocks, pl.prefix_chunk, pl.prefix_chunks);
+        split_keys(a->prefix_len, (int64_t) c->n_head_kv * pl.prefix_tiles, prefix_tc ? ctx->sm_count : blocks, prefix_tc ? tc_pass : pass, pl.prefix_chunk,
+                   pl.prefix_chunks);
     }
     const int64_t limit = (int64_t) 1 << 31;
     if ((int64_t) a->n_seq * c->n_head_kv * pl.own_tiles * pl.own_chunks >= limit || (int64_t) c->n_head_kv * pl.prefix_tiles * pl.prefix_chunks >= limit)
@@ -202,8 +210,11 @@ int launch_join(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t 
 
 namespace b200moe {
 extern template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+extern template int launch_attend_tc<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
 extern template int launch_attend<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+extern template int launch_attend_tc<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
 extern template int launch_attend<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
+extern template int launch_attend_tc<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
 }  // namespace b200moe
 
 extern "C" {
@@ -315,7 +326,8 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     p.q_start = a->q_start; p.kv_len = a->kv_len; p.pages = a->pages; p.prefix_pages = a->prefix_pages;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.own_chunk = pl.own_chunk; p.own_chunks = pl.own_chunks;
-    p.prefix_chunk = pl.prefix_chunk; p.prefix_chunks = pl.prefix_chunks;
+    p.prefix_chunk = pl.prefix_chunk; p.prefix_chunks = pl.prefix_chunks; p.own_prefix = pl.own_prefix;
+    p.q_aligned = rows_aligned(q); p.out_aligned = rows_aligned(out);
     p.direct = pl.bytes == 0;
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + pl.part_o);
@@ -323,16 +335,24 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     CUDA_TRY(ctx, cudaSetDevice(ctx->device));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto launch = [&](int nt, bool prefix, bool overlap, int blocks) {
-        if (cache->type == KV_BF16) return launch_attend<KV_BF16>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
-        if (cache->type == KV_Q8) return launch_attend<KV_Q8>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
-        return launch_attend<KV_Q4>(ctx, p, cache->head_dim, f32, nt, prefix, overlap, blocks, st);
+        const int d = cache->head_dim;
+        if (nt == TC_TILE) {
+            if (cache->type == KV_BF16) return launch_attend_tc<KV_BF16>(ctx, p, d, prefix, blocks, st);
+            if (cache->type == KV_Q8) return launch_attend_tc<KV_Q8>(ctx, p, d, prefix, blocks, st);
+            return launch_attend_tc<KV_Q4>(ctx, p, d, prefix, blocks, st);
+        }
+        if (cache->type == KV_BF16) return launch_attend<KV_BF16>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
+        if (cache->type == KV_Q8) return launch_attend<KV_Q8>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
+        return launch_attend<KV_Q4>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
     };
     if (pl.prefix_chunks) {
         p.row_tiles = pl.prefix_tiles;
         if (int rc = launch(pl.prefix_nt, true, false, pl.prefix_tiles * cache->n_head_kv * pl.prefix_chunks)) return rc;
     }
+    // nothing becomes resident beside a kernel that holds tensor memory
+    const bool overlap = pl.prefix_chunks > 0 && pl.prefix_nt != TC_TILE && pl.own_nt != TC_TILE;
     p.row_tiles = pl.own_tiles;
-    if (int rc = launch(pl.own_nt, false, pl.prefix_chunks > 0, pl.own_tiles * cache->n_head_kv * pl.own_chunks * a->n_seq)) return rc;
+    if (int rc = launch(pl.own_nt, false, overlap, pl.own_tiles * cache->n_head_kv * pl.own_chunks * a->n_seq)) return rc;
     if (p.direct) return B200MOE_OK;
     if (cache->head_dim == 64) return launch_join<64>(ctx, p, f32, st);
     if (cache->head_dim == 128) return launch_join<128>(ctx, p, f32, st);

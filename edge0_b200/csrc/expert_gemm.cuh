@@ -30,40 +30,12 @@
 
 namespace b200moe {
 
-__device__ __forceinline__ void mbar_arrive(uint64_t * bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // tiled 2-D TMA load (no multicast); x counts elements of the innermost dimension and must keep the copy 16-byte aligned
 __device__ __forceinline__ void tma_load_2d(void * dst_smem, const CUtensorMap * map, int x, int y, uint64_t * bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
                      smem_u32(dst_smem)),
                  "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
                  : "memory");
-}
-
-// Bounded wait that also returns when another role has given up; reports a timeout itself.
-// SLEEP_NS > 0: the warp sleeps between polls.  A polling warp otherwise competes for issue slots with the dequantising
-// warps of its scheduler (measured: more than half of all issued instructions were polls); roles that wait most of the
-// time (producers, epilogue, MMA issuer) therefore back off.
-template <int SLEEP_NS = 0>
-__device__ __forceinline__ bool wait_or_abort(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int * err) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t i = 0; i < (1u << 30); ++i) {
-        if (SLEEP_NS > 0) __nanosleep(SLEEP_NS);
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63) == 63) {
-            if (*abort_flag) return false;
-            if (global_timer_ns() - t0 > 2000000000ull) {
-                report_error(err, DEV_ERR_BARRIER_TIMEOUT);
-                *abort_flag = 1;
-                return false;
-            }
-        }
-    }
-    *abort_flag = 1;
-    return false;
 }
 
 // The shared-memory descriptor of umma_desc_k128 split into its constant high word and the low word without the address.

@@ -1,6 +1,5 @@
-// tcgen05 / TMEM building blocks of the tensor-core expert path: instruction wrappers, shared-memory and instruction
-// descriptors, the NVFP4 -> fp16 decode, and the kernel that prepares expert-sorted fp16 activations.
-// The grouped GEMM itself is in expert_gemm.cuh.
+// Building blocks of the tensor-core expert path: the NVFP4 -> fp16 decode, and the kernel that prepares expert-sorted fp16 activations.
+// The instruction wrappers and descriptors are in tensor_core.cuh, the grouped GEMM itself is in expert_gemm.cuh.
 //
 // Parity mode: activations stay on the reference's int8 grid (q * d, exactly what the CPU path multiplies with).  The
 // product q * d has up to 18 significant bits, so it is carried as TWO fp16 numbers hi + lo (exact for the fp16 block
@@ -18,63 +17,9 @@
 #include "common.cuh"
 #include "formats.cuh"
 #include "router.cuh"
+#include "tensor_core.cuh"
 
 namespace b200moe {
-
-// ---- tcgen05 / TMEM wrappers ---------------------------------------------------------------------------------
-__device__ __forceinline__ void tmem_alloc(uint32_t * smem_dst, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16, issued by one thread
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// all tcgen05 operations issued so far by this thread arrive on the mbarrier when they complete
-__device__ __forceinline__ void umma_commit(uint64_t * bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// 32 lanes x 16 consecutive 32-bit columns: thread i of the warp receives lane (base lane + i)
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Shared-memory matrix descriptor of a K-major tile with 128-byte rows, 128B swizzle, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_k128(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t) ((smem_addr >> 4) & 0x3fff);   // start address
-    d |= (uint64_t) 1 << 16;                        // leading byte offset (unused with swizzled K-major), 16-byte units
-    d |= (uint64_t) (1024 >> 4) << 32;              // stride byte offset between 8-row groups
-    d |= (uint64_t) 1 << 46;                        // descriptor version of this architecture
-    d |= (uint64_t) 2 << 61;                        // SWIZZLE_128B
-    return d;
-}
-// instruction descriptor: fp16 A and B, both K-major, fp32 accumulate, M = 128, N = n
-__device__ __forceinline__ uint32_t umma_idesc_f16(int n) { return (1u << 4) | ((uint32_t) (n >> 3) << 17) | ((128u >> 4) << 24); }
-
-// byte offset of 16-byte chunk c (0..7) of row r inside a [rows][64 halfs] tile laid out for SWIZZLE_128B
-__device__ __forceinline__ uint32_t sw128_offset(int r, int c) { return (uint32_t) ((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4)); }
 
 // ---- activations for the tensor-core path --------------------------------------------------------------------------
 // fp16(q * d) of the routed rows, gathered into expert order (row i of the output is routed row perm[i]) so every expert's

@@ -1,8 +1,8 @@
 """Attention over the paged cache (b200moe_attention) against softmax in 64 bits over the values that the cache holds (b200moe_kv_read).
 
 Tolerance, per output: half a step of the output's type relative to the value (bf16 2^-8, fp32 2^-24), plus the weights' errors times
-sum_j p_j |v_j|:  2 ds for the scores' errors ds (they act on numerator and sum alike), w for the weights' own rounding (one f16 2^-11, two
-bf16 2^-16, fp32 queries 2^-21 with the exponential's 2 ulp) and 2^-24 for each of about L / 64 + 64 additions.  ds = (D / 16 + 8) 2^-23 times the
+sum_j p_j |v_j|:  2 ds for the scores' errors ds (they act on numerator and sum alike), w for the weights' own rounding (to f16, 2^-11, for bf16
+queries; 2^-21 with the exponential's 2 ulp for fp32 ones) and 2^-24 for each of about L / 64 + 64 additions.  ds = (D / 16 + 8) 2^-23 times the
 largest scale sum |q| |k| of the row: a run of D / 16 instructions that drop at most the accumulator's last bit each, and a few roundings
 of the factors around it.  For bf16 queries the output accumulator, too, drops a last bit in each of its L / 64 steps: 2^-23 there."""
 import math
@@ -66,7 +66,7 @@ class Batch:
                     out[t] = torch.einsum("hk,khd->hd", p, w)
                     ds = (self.D / 16 + 8) * 2.0 ** -23 * (torch.einsum("hd,khd->hk", q.abs(), a.abs()).amax(-1) * abs(scale) + lse[t].abs())
                     f32 = self.dtype == torch.float32
-                    own = 2.0 ** -21 if f32 else 2.0 ** -11 if self.cache.kind == "q8" else 2.0 ** -16
+                    own = 2.0 ** -21 if f32 else 2.0 ** -11
                     weight = 2 * ds + own + (seen / 64 + 64) * (2.0 ** -24 if f32 else 2.0 ** -23)
                     tol[t] = weight[:, None] * torch.einsum("hk,khd->hd", p, w.abs()) + (2.0 ** -24 if f32 else 2.0 ** -8) * out[t].abs() + 1e-30
                 t += 1
