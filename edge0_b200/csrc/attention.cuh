@@ -225,7 +225,10 @@ __device__ __forceinline__ void load_values(ValueRegs<TYPE, D> & t, const KvView
     for (int i = 0; i < 2; ++i) load_scales<TYPE, D>(t.d[i], kv.v_scale, row0 + r + 8 * i);
 }
 
-// Operand A of the score product's k step: 16 keys by the 16 head_dim indexes key_dim() names
+// Operand A of the score product's k step: 16 keys by 16 head_dim indexes.  Lane column c's values v = 0, 1 (of the first 8 columns) and 2, 3 (of
+// the last) are index
+//   BF16  32 (step / 2) + 8c + 4 (step & 1) + v      Q8  64 (step / 4) + 16c + 4 (step & 3) + v
+//   Q4    32 (step / 2) + 8c + 2 (step & 1) + (v >> 1) + 4 (v & 1)
 template <int TYPE, int D>
 __device__ __forceinline__ void key_operand(uint32_t (&a)[4], const KeyRegs<TYPE, D> & t, int step) {
 #pragma unroll
@@ -243,14 +246,6 @@ __device__ __forceinline__ void key_operand(uint32_t (&a)[4], const KeyRegs<TYPE
         }
     }
 }
-// head_dim index of k step `step`, lane column c, value v: 0, 1 are the pair of the operand's first 8 columns, 2, 3 of the last
-template <int TYPE, int D>
-__device__ __forceinline__ int key_dim(int step, int c, int v) {
-    if (TYPE == KV_BF16) return 32 * (step / 2) + 8 * c + 4 * (step & 1) + v;
-    if (TYPE == KV_Q8) return 64 * (step / 4) + 16 * c + 4 * (step & 3) + v;
-    return 32 * (step / 2) + 8 * c + 2 * (step & 1) + (v >> 1) + 4 * (v & 1);
-}
-
 // Operand A of the output product's m tile: 16 head_dim indexes by 16 keys; lane row r is index value_dim(), row r + 8 the one behind it
 template <int TYPE, int D>
 __device__ __forceinline__ void value_operand(uint32_t (&a)[4], const ValueRegs<TYPE, D> & t, int tile) {
@@ -332,64 +327,6 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
     const int key_end = min(key0 + (PREFIX ? p.prefix_chunk : p.own_chunk), reach(n_rows - 1));
     const int seen_by_all = reach(0);
 
-    // the queries as operands, a row at a time per warp
-    for (int row = warp; row < S::ROWS; row += ATTN_WARPS) {
-        const bool there = row < n_rows;
-        const int token = there ? first + (row0 + row) / p.group : 0, h = there ? head * p.group + (row0 + row) % p.group : 0;
-        const XT * src = reinterpret_cast<const XT *>(p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head);
-        float up = 1.0f, factor = p.scale_log2;
-        if (!S::BF) {
-            float m = 0.0f;
-            if (there)
-                for (int i = lane; i < D; i += 32) m = fmaxf(m, fabsf(to_float(src[i])));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int e = min(max((int) (__float_as_uint(m) >> 23), 40), 250);    // 2^(e - 127) <= m, kept where both powers are normal
-            up = __uint_as_float((uint32_t) (254 + 14 - e) << 23);
-            factor = p.scale_log2 / up;
-        }
-        if (lane == 0) {
-            s_factor[row] = factor;
-            s_seen[row] = there ? reach(row) : 0;
-        }
-        // word (term, step, row / 8, lane, half) of the operand; lane (row % 8, c)
-        for (int e = lane; e < S::STEPS * 8; e += 32) {
-            const int half = e & 1, cc = (e >> 1) & 3, step = e >> 3;
-            float x = 0.0f, y = 0.0f;
-            if (there) {
-                x = to_float(src[key_dim<TYPE, D>(step, cc, 2 * half)]) * up;
-                y = to_float(src[key_dim<TYPE, D>(step, cc, 2 * half + 1)]) * up;
-            }
-            uint32_t terms[S::QT];
-            split2<S::BF, S::QT>(x, y, terms);
-#pragma unroll
-            for (int n = 0; n < S::QT; ++n) sq[(((n * S::STEPS + step) * NT + row / 8) * 32 + (row % 8) * 4 + cc) * 2 + half] = terms[n];
-        }
-    }
-    __syncthreads();
-    float factor[NT][2];
-    int seen[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            factor[n][i] = s_factor[8 * n + 2 * c + i];
-            seen[n][i] = s_seen[8 * n + 2 * c + i];
-        }
-
-    float o[S::STEPS][NT][4], m[NT][2], l[NT][2];
-    int top[NT][2];    // Q8: exponent bits of the largest value scale that the row has seen, 2^-100 at least
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) { m[n][i] = -INFINITY; l[n][i] = 0.0f; top[n][i] = 27 << 23; }
-#pragma unroll
-    for (int t = 0; t < S::STEPS; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][n][i] = 0.0f;
-
     const int32_t * table = PREFIX ? p.prefix_pages : p.pages + (int64_t) seq * p.pages_stride;
     const int shift = p.kv.page_shift, in_page = (1 << shift) - 1, n_pages = (int) (p.kv.n_slots >> shift);
     constexpr int STRIDE = 16 * S::KS * ATTN_WARPS;
@@ -421,6 +358,80 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
             load_values<TYPE, D>(vr[j], p.kv, row, lane);
         }
     }
+    // ---- the queries as operands, eight values to a thread at a time; the first keys and values are on their way
+    {
+        constexpr int TPR = D / 8, PASS = 32 * ATTN_WARPS / TPR;
+        const int i = threadIdx.x % TPR;
+        float x[(S::ROWS + PASS - 1) / PASS][8];
+#pragma unroll
+        for (int n = 0; n < (S::ROWS + PASS - 1) / PASS; ++n) {
+            const int row = n * PASS + threadIdx.x / TPR;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[n][j] = 0.0f;
+            if (row < n_rows) {
+                const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
+                load8<XT>(x[n], p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head, i, p.q_aligned);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < (S::ROWS + PASS - 1) / PASS; ++n) {
+            const int row = n * PASS + threadIdx.x / TPR;
+            float up = 1.0f, factor = p.scale_log2;
+            if (!S::BF) {
+                float m = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[n][j]));
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                const int e = min(max((int) (__float_as_uint(m) >> 23), 40), 250);    // 2^(e - 127) <= m, kept where both powers are normal
+                up = __uint_as_float((uint32_t) (254 + 14 - e) << 23);
+                factor = p.scale_log2 / up;
+            }
+            if (S::ROWS % PASS == 0 || row < S::ROWS) {
+                if (i == 0) {
+                    s_factor[row] = factor;
+                    s_seen[row] = row < n_rows ? reach(row) : 0;
+                }
+                // values 8i .. 8i + 7 are steps s0, s0 + 1 of lane column cc (key_operand())
+                const int s0 = TYPE == KV_Q8 ? 4 * (i / 8) + 2 * (i & 1) : 2 * (i / 4), cc = TYPE == KV_Q8 ? (i % 8) / 2 : i % 4;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int lo = TYPE == KV_Q4 ? 2 * u + half : 4 * u + 2 * half, hi = TYPE == KV_Q4 ? lo + 4 : lo + 1;
+                        uint32_t terms[S::QT];
+                        split2<S::BF, S::QT>(x[n][lo] * up, x[n][hi] * up, terms);
+#pragma unroll
+                        for (int v = 0; v < S::QT; ++v)
+                            sq[(((v * S::STEPS + s0 + u) * NT + row / 8) * 32 + (row % 8) * 4 + cc) * 2 + half] = terms[v];
+                    }
+            }
+        }
+    }
+    __syncthreads();
+    float factor[NT][2];
+    int seen[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            factor[n][i] = s_factor[8 * n + 2 * c + i];
+            seen[n][i] = s_seen[8 * n + 2 * c + i];
+        }
+
+    float o[S::STEPS][NT][4], m[NT][2], l[NT][2];
+    int top[NT][2];    // Q8: exponent bits of the largest value scale that the row has seen, 2^-100 at least
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { m[n][i] = -INFINITY; l[n][i] = 0.0f; top[n][i] = 27 << 23; }
+#pragma unroll
+    for (int t = 0; t < S::STEPS; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][n][i] = 0.0f;
+
     for (; key < key_end; key += STRIDE) {
         // ---- scores: 16 keys by 8 NT rows; lane has keys r, r + 8 and rows 2c, 2c + 1
         float s[S::KS][NT][4];
@@ -705,15 +716,19 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
     }
 }
 
-// joins the chunks of a (token, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c
-template <int D, typename XT>
-__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr int WARPS = 4, PER = D / 32;
-    __shared__ float so[WARPS][D];
-    __shared__ float2 sml[WARPS];
+// Joins the chunks of a (token, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.  WARPS warps to a row: one where there are few chunks,
+// eight with their loads in flight together where a long axis was cut into many (a document of 131072 keys, 205 chunks: 30 us with
+// four warps that each read a chunk's maximum before its outputs, 6 now).
+constexpr int JOIN_THREADS = 256, JOIN_CHUNKS = 1024;
+template <int D, typename XT, int WARPS>
+__global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ AttnParams p) {
+    constexpr int PER = D / 32, LINES = JOIN_THREADS / 32 / WARPS, MOST = WARPS == 1 ? 32 : JOIN_CHUNKS;
+    __shared__ float s_weight[LINES][MOST];
+    __shared__ float s_sum[WARPS], s_most[WARPS];
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t line = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WARPS == 1 ? warp : 0, part = WARPS == 1 ? 0 : warp;
+    const int64_t line = (int64_t) blockIdx.x * LINES + sub;
+    if (line >= (int64_t) p.n_tokens * p.n_head) return;    // whole warps, of which none waits for another (LINES is 1 where they do)
     const int token = (int) (line / p.n_head);
     int seq = token;
     if (p.q_start) {    // the last sequence that begins at or before the token
@@ -728,45 +743,69 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
     int first, n_new, len;
     if (seq >= p.n_seq || !attn_sequence(p, seq, first, n_new, len, false) || token < first || token >= first + n_new) return;    // a row that belongs to nobody
     const int reach = p.own_prefix + max(0, len - n_new + (token - first) + 1);
-    const int own = p.own_chunks ? (reach + p.own_chunk - 1) / p.own_chunk : 0;
+    const int own = (reach + p.own_chunk - 1) / p.own_chunk;
     const int n = p.prefix_chunks + own, chunks = p.prefix_chunks + p.own_chunks;
     const float2 * ml = p.part_ml + line * chunks;
     const float * o = p.part_o + line * chunks * D;
-    float most = -INFINITY;
-    for (int i = lane; i < n; i += 32) most = fmaxf(most, ml[i].x);
+    // ---- the chunks' weights
+    float most = -INFINITY, sum = 0.0f;
+    for (int i = part * 32 + lane; i < n; i += 32 * WARPS) most = fmaxf(most, ml[i].x);
 #pragma unroll
     for (int x = 16; x > 0; x /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
-    float acc[PER], sum = 0.0f;
+    if (WARPS > 1) {
+        if (lane == 0) s_most[part] = most;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (int i = warp; i < n; i += WARPS) {
+        for (int w = 0; w < WARPS; ++w) most = fmaxf(most, s_most[w]);
+    }
+    for (int i = part * 32 + lane; i < n; i += 32 * WARPS) {
         const float2 x = ml[i];
         const float f = x.x == -INFINITY ? 0.0f : fast_exp2(x.x - most);
-        const Pack<float, PER> v = *reinterpret_cast<const Pack<float, PER> *>(o + (int64_t) i * D + lane * PER);
-        if (x.x != -INFINITY || x.y != 0.0f) {
-            sum += x.y * f;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) acc[j] += v.v[j] * f;
-        }
+        const bool some = x.x != -INFINITY || x.y != 0.0f;
+        s_weight[sub][i] = some ? f : -1.0f;    // nothing there: the outputs are not to be looked at
+        if (some) sum += x.y * f;
     }
 #pragma unroll
-    for (int j = 0; j < PER; ++j) so[warp][lane * PER + j] = acc[j];
-    if (lane == 0) sml[warp] = make_float2(most, sum);
-    __syncthreads();
-    sum = 0.0f;
+    for (int x = 16; x > 0; x /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (WARPS > 1) {
+        if (lane == 0) s_sum[part] = sum;
+        __syncthreads();
+        sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) sum += sml[w].y;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int w = 0; w < WARPS; ++w) sum += s_sum[w];
+    } else {
+        __syncwarp();
+    }
+    // ---- their outputs
+    float acc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+#pragma unroll 8
+    for (int i = part; i < n; i += WARPS) {
+        const Pack<float, PER> v = *reinterpret_cast<const Pack<float, PER> *>(o + (int64_t) i * D + lane * PER);
+        const float f = s_weight[sub][i];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) acc[j] += f < 0.0f ? 0.0f : v.v[j] * f;
+    }
     const int h = (int) (line % p.n_head);
     XT * dst = reinterpret_cast<XT *>(p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head);
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float x = 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if constexpr (WARPS == 1) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) x += so[w][d];
-        dst[d] = from_float<XT>(x * inv);
+        for (int j = 0; j < PER; ++j) dst[lane * PER + j] = from_float<XT>(acc[j] * inv);
+    } else {
+        __shared__ float so[WARPS][D];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) so[part][lane * PER + j] = acc[j];
+        __syncthreads();
+        for (int d = threadIdx.x; d < D; d += JOIN_THREADS) {
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) x += so[w][d];
+            dst[d] = from_float<XT>(x * inv);
+        }
     }
-    if (p.lse && threadIdx.x == 0) p.lse[line] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
+    if (p.lse && part == 0 && lane == 0) p.lse[line] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
 }
 
 // One launch for the own keys or the prefix; the kernels are in a translation unit for each type of cache.  nt: rows to a tile / 8, 1, 2 or 4
@@ -774,7 +813,8 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant_
 template <int TYPE>
 int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st);
 
-// The same for bf16 queries and tiles of 128 rows (attention_tc.cuh), a launch of its own in every case.
+// The same for bf16 queries and tiles of attend_tc_rows() rows (attention_tc.cuh), a launch of its own in every case.
+__host__ __device__ constexpr int attend_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 template <int TYPE>
 int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, int blocks, cudaStream_t st);
 

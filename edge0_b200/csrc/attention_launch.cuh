@@ -68,8 +68,8 @@ int launch_attend_tc_t(ContextBase * ctx, const AttnParams & p, int blocks, cuda
     constexpr size_t smem = TcShape<TYPE, D>::SMEM;
     static bool done[ATTN_MAX_DEVICES] = {};
     if (int rc = raise_shared_limit(ctx, kern, smem, done)) return rc;
-    kern<<<(unsigned) blocks, TC_THREADS, smem, st>>>(p);
-    return check_launch(ctx, "attention, 128 rows to a tile");
+    kern<<<(unsigned) blocks, TcShape<TYPE, D>::THREADS, smem, st>>>(p);
+    return check_launch(ctx, "attention, tiles of many rows");
 }
 
 template <int TYPE>

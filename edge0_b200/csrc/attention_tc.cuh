@@ -1,43 +1,54 @@
-// Attention of many query rows to a key/value head (a shared prefix read by a whole batch, chunks of prompts) on tcgen05: 128 rows to a block,
-// keys in tiles of 128 (head_dim 256: 64), scores and outputs in tensor memory.  The same contract as attend_kernel (attention.cuh) for
-// bf16 queries; which of the two runs is decided by the rows (decoder_ops.cu).
+// Attention of many query rows to a key/value head (a shared prefix read by a whole batch, chunks of prompts) on tcgen05: two groups of 128 rows to a
+// block (head_dim 256: one), keys in tiles of 64, scores, weights and outputs in tensor memory.  The same contract as attend_kernel
+// (attention.cuh) for bf16 queries; which of the two runs is decided by the rows (decoder_ops.cu).
 //
-// Roles, meeting at mbarriers (every wait is bounded; two stages of keys, values, scores and weights):
-//   warps 0-7    softmax: a thread has half of the tile's keys of one row (a warp reads the 32 tensor-memory lanes of its rank in its warpgroup), takes the
-//                maximum with its partner of the other half, writes the weights to tensor memory as f16, scales the outputs back when the
-//                reference has to rise, and at the end reads them out
-//   warps 8-15   producers: cache rows through registers into f16 operand tiles (128B swizzle), the next tile's loads in flight meanwhile
-//   warp 16      one thread issues S = Q K^T (both operands from shared memory) and O += P V (P from tensor memory, V as it lies, head_dim contiguous)
+// Roles, meeting at mbarriers (every wait is bounded):
+//   warps 0 .. 4 G - 1   softmax, four warps to a group: a thread owns a row (its tensor-memory lane).  It takes a tile's 64 scores into registers and
+//                        writes the weights back over them as f16 pairs; when the reference has to rise it scales the row's outputs
+//                        back; at the end it reads the outputs out
+//   four warps           producers: cache rows through registers into f16 operand tiles (128B swizzle, two to four stages), the next tile's loads in flight
+//   two threads a group  issue S = Q K^T (both operands from shared memory) and O += P V (P from tensor memory, V as it lies, head_dim contiguous).
+//                        An instruction holds its thread about 75 cycles whatever its size, and a commit more: one thread for all took
+//                        3,300 cycles to a tile.  Every group has two buffers of scores, so that the next tile's are ready when a tile's softmax ends
 //
 // Precision.  Every operand is f16 and every factor a power of two or outside: rows of Q and of BF16 and Q4 caches are brought to the same size by a power of
 // two a row (bf16's 8 bits, and a 3-bit code times an 8-bit scale, fit f16's 11), Q8 codes are whole numbers; a key's factor multiplies its score,
 // a value's its weight, in fp32.  The weights 2^(s - ref) times the values' factors are rounded to f16 (2^-11).  ref rises only when a tile's
 // maximum is more than 2^8 above it: weights stay below 2^15, sums are fp32.
 //
-// Bound by the issue of the softmax and the conversion: 128 x 128 scores cost about 6.5 instructions each, 32 K values about 1.2 (Q8), together 1,300 cycles
-// of a scheduler, where the two products need 1,024 of the tensor pipe.
+// Bound by the exponentials (16 a cycle and SM: 1,024 cycles for 64 keys of 256 rows), the products (about 1,200 cycles with operands read
+// from shared memory at 128 bytes a cycle) and issue (a score costs about five instructions, packed fp32 pairs where there are such; a value of
+// the cache 1.2 (Q8) to 2.5 (BF16), shared by the block's 256 rows).
 #pragma once
 #include "attention.cuh"
 #include "tensor_core.cuh"
 
 namespace b200moe {
 
-constexpr int TC_SOFTMAX_WARPS = 8, TC_PRODUCER_WARPS = 8;
-constexpr int TC_THREADS = 32 * (TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS + 1);
-constexpr int TC_ROWS = 128;
+constexpr int TC_GROUP_ROWS = 128;
+constexpr int TC_PRODUCER_WARPS = 4;
+constexpr int TC_KEYS = 64;    // to a tile
+
+// rows to a block
+__host__ __device__ constexpr int tc_rows(int head_dim) { return attend_tc_rows(head_dim); }
 
 template <int TYPE, int D>
 struct TcShape {
-    static constexpr int KT = D == 256 ? 64 : 128;                                     // keys to a tile
+    static constexpr int GROUPS = tc_rows(D) / TC_GROUP_ROWS;
+    static constexpr int SOFTMAX_WARPS = 4 * GROUPS;
+    static constexpr int ISSUE_WARPS = 2 * GROUPS;                                     // scores and outputs of each group
+    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + TC_PRODUCER_WARPS + ISSUE_WARPS);
     static constexpr int VALUES = TYPE == KV_BF16 ? 8 : TYPE == KV_Q8 ? 16 : 32;       // of a row in a producer's 16 bytes
     static constexpr int TPR = D / VALUES;                                             // producers to a row
     static constexpr int ROWS = 32 * TC_PRODUCER_WARPS / TPR;                          // rows to a pass of all producers
-    static constexpr int NL = KT / ROWS;                                               // passes
-    static constexpr int Q_BYTES = TC_ROWS * D * 2, KV_BYTES = KT * D * 2;
-    static constexpr uint32_t T_S = 0, T_O = 2 * KT, T_P = T_O + D;                    // tensor-memory columns: scores (2), outputs, weights (2)
-    static constexpr size_t SMEM = Q_BYTES + 4 * KV_BYTES + 1024;
-    static_assert(T_P + KT <= 512, "tensor memory");
-    static_assert(ROWS * NL == KT, "tile");
+    static constexpr int PARTS = TC_KEYS / ROWS > 8 ? TC_KEYS / ROWS / 8 : 1;          // a tile goes through registers in so many parts
+    static constexpr int NL = TC_KEYS / ROWS / PARTS;                                  // passes of a part
+    static constexpr int STAGES = D == 256 ? 2 : 4;                                    // of keys and of values
+    static constexpr int Q_BYTES = TC_GROUP_ROWS * D * 2, KV_BYTES = TC_KEYS * D * 2;  // Q_BYTES: of a group
+    static constexpr uint32_t T_S = 0, T_O = 2 * GROUPS * TC_KEYS;                     // tensor-memory columns: scores and weights (2 a group), outputs
+    static constexpr size_t SMEM = GROUPS * Q_BYTES + 2 * STAGES * KV_BYTES + 1024;
+    static_assert(T_O + GROUPS * D <= 512, "tensor memory");
+    static_assert(NL >= 1 && ROWS * NL * PARTS == TC_KEYS, "tile");
 };
 
 // D[tmem] (+)= A[tmem, 16-bit pairs in a column] * B[smem desc]
@@ -49,25 +60,100 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// 32 lanes x N columns, without a wait
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t * r) {
-    static_assert(N == 16, "pieces of 16 columns");
+// 32 lanes x 16 or 32 columns, without a wait
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t * r) {
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
           "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+          "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+          "r"(r[30]), "r"(r[31])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// As wait_or_abort (tensor_core.cuh), with the thread suspended by the hardware for up to 20 us at a time: polls of the roles that wait
+// most of the time would take issue slots from the softmax.
+__device__ __forceinline__ bool wait_suspended(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int * err) {
+    auto attempt = [&]() {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+        return ok != 0;
+    };
+    if (attempt()) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t i = 0; i < (1u << 30); ++i) {
+        if (attempt()) return true;
+        if (*abort_flag) return false;
+        if ((i & 15) == 15 && global_timer_ns() - t0 > 2000000000ull) break;
+    }
+    report_error(err, DEV_ERR_BARRIER_TIMEOUT);
+    *abort_flag = 1;
+    return false;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// two fp32 operations to an instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
 // byte offset of 16-byte piece `chunk` of row `row` in a tile of `rows` rows of head_dim f16 values: blocks of 64 values, 128 bytes a row, swizzled
 __device__ __forceinline__ uint32_t tc_offset(int rows, int row, int chunk) {
@@ -102,16 +188,17 @@ struct TcPiece {
 };
 
 template <int TYPE, int D>
-__device__ __forceinline__ void tc_load(TcPiece<TYPE, D> & t, const uint8_t * rows, const void * scales, const int64_t * row, int x) {
+__device__ __forceinline__ void tc_load(TcPiece<TYPE, D> & t, const uint8_t * rows, const void * scales, const KvView & kv, const int * slot, int head, int x) {
     typedef TcShape<TYPE, D> S;
 #pragma unroll
     for (int n = 0; n < S::NL; ++n) {
         t.v[n] = make_uint4(0, 0, 0, 0);
-        if (row[n] >= 0) t.v[n] = load_stream(reinterpret_cast<const uint4 *>(rows + row[n] * kv_row_bytes<TYPE, D>() + 16 * x));
-        if (TYPE == KV_Q8) t.s[n][0] = row[n] >= 0 ? static_cast<const uint32_t *>(scales)[row[n]] : 0u;
+        const int64_t row = kv_row(kv, max(slot[n], 0), head);
+        if (slot[n] >= 0) t.v[n] = load_stream(reinterpret_cast<const uint4 *>(rows + row * kv_row_bytes<TYPE, D>() + 16 * x));
+        if (TYPE == KV_Q8) t.s[n][0] = slot[n] >= 0 ? static_cast<const uint32_t *>(scales)[row] : 0u;
         if (TYPE == KV_Q4)
 #pragma unroll
-            for (int g = 0; g < D / 64; ++g) t.s[n][g] = row[n] >= 0 ? static_cast<const uint32_t *>(scales)[row[n] * (D / 64) + g] : 0u;
+            for (int g = 0; g < D / 64; ++g) t.s[n][g] = slot[n] >= 0 ? static_cast<const uint32_t *>(scales)[row * (D / 64) + g] : 0u;
     }
 }
 
@@ -132,8 +219,8 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
         hi = make_uint4(h[4], h[5], h[6], h[7]);
         // the threads of a row's second 64 values begin with the other piece: their block lies on the same banks
         const int first = (x >> 2) & 1;
-        *reinterpret_cast<uint4 *>(tile + tc_offset(S::KT, row, 2 * x + first)) = first ? hi : lo;
-        *reinterpret_cast<uint4 *>(tile + tc_offset(S::KT, row, 2 * x + 1 - first)) = first ? lo : hi;
+        *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, 2 * x + first)) = first ? hi : lo;
+        *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, 2 * x + 1 - first)) = first ? lo : hi;
         return __uint_as_float(t.s[n][0]);
     } else if (TYPE == KV_Q4) {
         constexpr int GB = D >= 128 ? 4 : 2;
@@ -177,7 +264,7 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
                 const __half2 v = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&u), __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408))), s2);
                 h[j] = zero ? 0u : half2_bits(v);
             }
-            *reinterpret_cast<uint4 *>(tile + tc_offset(S::KT, row, 4 * (run * GB + g) + c)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, 4 * (run * GB + g) + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         return clean && !finite ? __uint_as_float(0x7fffffffu) : pow2_inverse(up);
     } else {
@@ -193,23 +280,24 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             h[i] = zero ? 0u : half2_bits(__floats2half2_rn(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up));
-        *reinterpret_cast<uint4 *>(tile + tc_offset(S::KT, row, x)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, x)) = make_uint4(h[0], h[1], h[2], h[3]);
         return zero ? __uint_as_float(0x7fffffffu) : pow2_inverse(up);
     }
 }
 
 template <int TYPE, int D, bool PREFIX>
-__global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel(const __grid_constant__ AttnParams p) {
     typedef TcShape<TYPE, D> S;
-    constexpr int KT = S::KT, HALF = KT / 2;
+    constexpr int KT = TC_KEYS, NS = S::STAGES, GROUPS = S::GROUPS, SW = S::SOFTMAX_WARPS;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t * sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t) 1023);
-    uint8_t * sk = sq + S::Q_BYTES, * sv = sk + 2 * S::KV_BYTES;
-    __shared__ uint64_t k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], s_free[2], p_full[2], pv_done[2], met[4];
-    __shared__ __align__(16) float k_scale[2][KT], v_scale[2][KT];
-    __shared__ float2 other[2][2][TC_ROWS];    // what the two threads of a row tell one another
-    __shared__ float s_factor[TC_ROWS];
-    __shared__ int s_bad[2];
+    uint8_t * sk = sq + GROUPS * S::Q_BYTES, * sv = sk + NS * S::KV_BYTES;
+    __shared__ uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS];
+    __shared__ uint64_t q_full, s_full[2 * GROUPS], p_full[2 * GROUPS], pv_done[2 * GROUPS];    // [group][parity of the tile]
+    __shared__ __align__(16) float k_scale[NS][KT], v_scale[NS][KT];
+    __shared__ float s_factor[GROUPS * TC_GROUP_ROWS];
+    __shared__ int s_bad[NS];
+    __shared__ __align__(16) float v_top[NS][TC_PRODUCER_WARPS];    // the largest of the values' factors that a producer warp has seen in the tile
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_abort;
 
@@ -229,340 +317,388 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
     } else if (!attn_sequence(p, seq, first, n_new, len, tid == 0 && row_tile == 0 && head == 0 && chunk == 0)) {
         return;
     }
-    const int row0 = row_tile * TC_ROWS, n_rows = min(n_new * p.group - row0, TC_ROWS);
+    const int row0 = row_tile * tc_rows(D), n_rows = min(n_new * p.group - row0, tc_rows(D));
     const int per_chunk = PREFIX ? p.prefix_chunk : p.own_chunk, key0 = chunk * per_chunk;
     if (n_rows <= 0 || (key0 >= front + len && !(key0 == 0 && p.direct))) return;
     auto reach = [&](int row) { return PREFIX ? front : front + max(0, len - n_new + (row0 + row) / p.group + 1); };
-    const int key_end = min(key0 + per_chunk, reach(n_rows - 1)), seen_by_all = reach(0);
+    const int key_end = min(key0 + per_chunk, reach(n_rows - 1));
     const int n_tiles = key_end > key0 ? (key_end - key0 + KT - 1) / KT : 0;
-    // some row does not see all keys of the tile (rows behind n_rows are nobody's)
-    auto masked_tile = [&](int i) { return key0 + (i + 1) * KT > min(seen_by_all, key_end); };
+    const int n_groups = GROUPS == 2 && n_rows > TC_GROUP_ROWS ? 2 : 1;
+    // some row from `row` on does not see all keys of the tile (rows behind n_rows are nobody's)
+    auto masked_tile = [&](int i, int row) { return key0 + (i + 1) * KT > min(reach(row), key_end); };
 
     if (tid == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 32 * TC_PRODUCER_WARPS);
             mbar_init(&v_full[i], 32 * TC_PRODUCER_WARPS);
-            mbar_init(&k_free[i], 1 + TC_SOFTMAX_WARPS);
-            mbar_init(&v_free[i], 1 + TC_SOFTMAX_WARPS);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&s_free[i], 32 * TC_SOFTMAX_WARPS);
-            mbar_init(&p_full[i], 32 * TC_SOFTMAX_WARPS);
-            mbar_init(&pv_done[i], 1);
+            mbar_init(&k_free[i], 5 * n_groups);    // a commit and four softmax warps of each group
+            mbar_init(&v_free[i], 5 * n_groups);
             s_bad[i] = 0;
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&met[i], 2);
+        for (int i = 0; i < 2 * GROUPS; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], TC_GROUP_ROWS);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(&q_full, 32 * SW);
         mbar_fence_init();
         s_abort = 0;
     }
-    if (warp == TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS) {
+    if (warp == SW + TC_PRODUCER_WARPS) {
         tmem_alloc(&s_tmem, 512);
         tmem_relinquish();
-    }
-    // ---- the queries: D / 8 threads to a row
-    {
-        constexpr int TPR = D / 8, PASS = 32 * (TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS) / TPR;
-        const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-        if (warp < TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS) {
-#pragma unroll
-            for (int r0 = 0; r0 < TC_ROWS; r0 += PASS) {
-                const int row = r0 + tid / TPR, x = tid % TPR;
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-                if (row < n_rows) {
-                    const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
-                    load8<__nv_bfloat16>(v, p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head, x, p.q_aligned);
-                }
-                float most = 0.0f;    // NaN says nothing about the size
-#pragma unroll
-                for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
-#pragma unroll
-                for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float up = row_up(__float_as_uint(most));
-                uint32_t h2[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h2[i] = half2_bits(__floats2half2_rn(v[2 * i] * (up * sign), v[2 * i + 1] * (up * sign)));
-                *reinterpret_cast<uint4 *>(sq + tc_offset(TC_ROWS, row, x)) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
-                if (x == 0) s_factor[row] = fabsf(p.scale_log2) * pow2_inverse(up);
-            }
-        }
-        fence_async_smem();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    if (warp < TC_SOFTMAX_WARPS) {
+    if (warp < SW) {
         // ------------------------------------------------------------ softmax
-        const int row = (warp & 3) * 32 + lane, half = warp >> 2;
-        const uint32_t t_lane = tmem + ((uint32_t) ((warp & 3) * 32) << 16);
-        const float factor = s_factor[row];
-        const int seen = reach(min(row, n_rows - 1));
-        float ref = -INFINITY, sum = 0.0f;
-        bool ok = true;
-        for (int i = 0; i < n_tiles; ++i) {
-            const int st = i & 1;
-            const uint32_t ph = (i >> 1) & 1;
-            // the votes reconverge the warp and make the outcome uniform for the instructions that need all of it
-            ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[st], ph, &s_abort, p.err) && wait_or_abort(&k_full[st], ph, &s_abort, p.err));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[HALF];
-#pragma unroll
-            for (int c = 0; c < HALF; c += 16) tmem_load<16>(t_lane + S::T_S + st * KT + half * HALF + c, s + c);
-            tmem_wait_ld();
-            tc_fence_before();
-            mbar_arrive(&s_free[st]);
-            const bool masked = masked_tile(i) || s_bad[st] == i + 1;
-            const int key = key0 + i * KT + half * HALF;
-            const float4 * ks = reinterpret_cast<const float4 *>(k_scale[st] + half * HALF);
-            float most = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < HALF; c += 4) {
-                const float4 f = ks[c / 4];
-                const float ff[4] = { f.x, f.y, f.z, f.w };
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float v = __uint_as_float(s[c + j]) * ff[j];
-                    s[c + j] = __float_as_uint(v);
-                    if (!masked) most = fmaxf(most, v);
-                }
-            }
-            uint64_t on = ~0ull;    // keys that the row sees
-            if (masked) {
-                on = 0;
-#pragma unroll
-                for (int c = 0; c < HALF; ++c) {
-                    // a negative factor marks a page that is not there
-                    const bool see = key + c < seen && !(k_scale[st][half * HALF + c] < 0.0f);
-                    if (see) { on |= 1ull << c; most = fmaxf(most, __uint_as_float(s[c])); }
-                }
-            }
-            ok = __all_sync(0xffffffffu, wait_or_abort(&v_full[st], ph, &s_abort, p.err));    // the values' factors
-            if (!ok) break;
-            if (lane == 0) mbar_arrive(&k_free[st]);
-            float top = 0.0f;    // the largest of the values' factors
-            if (!masked) {
-#pragma unroll
-                for (int c = lane; c < KT; c += 32) top = fmaxf(top, v_scale[st][c]);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            } else {
-#pragma unroll
-                for (int c = 0; c < HALF; ++c) if (on >> c & 1) top = fmaxf(top, v_scale[st][half * HALF + c]);
-            }
-            other[st][half][row] = make_float2(most, top);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&met[warp & 3]);
-            ok = __all_sync(0xffffffffu, wait_or_abort(&met[warp & 3], i & 1, &s_abort, p.err));
-            if (!ok) break;
-            const float2 partner = other[st][half ^ 1][row];
-            most = fmaxf(most, partner.x);
-            top = fmaxf(top, partner.y);
-            // weights 2^(s - ref) times a factor stay below 2^7 at this reference, and below 2^15 until it has to rise
-            const int e = max((int) (__float_as_uint(top) >> 23), 47);
-            const float want = most == -INFINITY ? -INFINITY : most * factor + (float) (e - 127 - 6);
-            const bool rise = want > ref + 8.0f || (ref == -INFINITY && want > -INFINITY);
-            if (__any_sync(0xffffffffu, rise)) {
-                const float back = !rise ? 1.0f : ref == -INFINITY ? 0.0f : fast_exp2(ref - want);
-                if (rise) { sum *= back; ref = want; }
-                if (i > 0) {
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[st ^ 1], ((i - 1) >> 1) & 1, &s_abort, p.err));
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int c = 0; c < D / 2; c += 16) {
-                        uint32_t o[16];
-                        tmem_load<16>(t_lane + S::T_O + half * (D / 2) + c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
-                        tmem_store16(t_lane + S::T_O + half * (D / 2) + c, o);
-                    }
-                    tmem_wait_st();
-                }
-            }
-            const float base = ref == -INFINITY ? 0.0f : ref;
-            const float4 * vs = reinterpret_cast<const float4 *>(v_scale[st] + half * HALF);
-            uint32_t w[HALF / 2];
-#pragma unroll
-            for (int c = 0; c < HALF; c += 4) {
-                const float4 f = vs[c / 4];
-                const float ff[4] = { f.x, f.y, f.z, f.w };
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float e2 = fast_exp2(fmaf(__uint_as_float(s[c + j]), factor, -base));
-                    x[j] = e2 * ff[j];
-                    if (masked && !(on >> (c + j) & 1)) { e2 = 0.0f; x[j] = 0.0f; }
-                    sum += e2;
-                }
-                w[c / 2] = half2_bits(__floats2half2_rn(x[0], x[1]));
-                w[c / 2 + 1] = half2_bits(__floats2half2_rn(x[2], x[3]));
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_free[st]);
-            // the weights' columns are free once the product two tiles back has read them
-            ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[st], ph ^ 1u, &s_abort, p.err));
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < HALF / 2; c += 16) tmem_store16(t_lane + S::T_P + st * (KT / 2) + half * (HALF / 2) + c, w + c);
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[st]);
-        }
-        // ---- the outputs
-        if (ok && n_tiles) ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, &s_abort, p.err));
-        tc_fence_after();
-        other[n_tiles & 1][half][row] = make_float2(sum, 0.0f);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&met[warp & 3]);
-        if (ok) ok = __all_sync(0xffffffffu, wait_or_abort(&met[warp & 3], n_tiles & 1, &s_abort, p.err));
-        if (ok) {
-            sum += other[n_tiles & 1][half ^ 1][row].x;
-            const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
-            const int64_t line = (int64_t) token * p.n_head + h;
-            const int chunks = p.prefix_chunks + p.own_chunks, slot = PREFIX ? chunk : p.prefix_chunks + chunk;
-            const float inv = p.direct ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-            const bool there = row < n_rows;
+        // ---- the queries: D / 8 threads to a row, the loads of several rows in flight together
+        constexpr int TPR = D / 8, PASS = 32 * SW / TPR, BATCH = GROUPS * TC_GROUP_ROWS / PASS < 16 ? GROUPS * TC_GROUP_ROWS / PASS : 16;
+        const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        const int x = tid % TPR;
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
-                uint32_t o[16];
-                if (n_tiles) {
-                    tmem_load<16>(t_lane + S::T_O + half * (D / 2) + c, o);
-                    tmem_wait_ld();
+        for (int r0 = 0; r0 < GROUPS * TC_GROUP_ROWS; r0 += PASS * BATCH) {
+            uint4 raw[BATCH];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const int row = r0 + n * PASS + tid / TPR, at_row = row0 + min(row, n_rows - 1);
+                const int token = first + at_row / p.group, h = head * p.group + at_row % p.group;
+                const char * src = p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head + 16 * x;
+                if (p.q_aligned) {
+                    raw[n] = *reinterpret_cast<const uint4 *>(src);
+                } else {
+                    const uint16_t * e = reinterpret_cast<const uint16_t *>(src);
+                    raw[n] = make_uint4(e[0] | (uint32_t) e[1] << 16, e[2] | (uint32_t) e[3] << 16, e[4] | (uint32_t) e[5] << 16, e[6] | (uint32_t) e[7] << 16);
+                }
+                if (row >= n_rows) raw[n] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const int row = r0 + n * PASS + tid / TPR;
+                const uint32_t w[4] = { raw[n].x, raw[n].y, raw[n].z, raw[n].w };
+                float most = 0.0f;    // NaN says nothing about the size
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+#pragma unroll
+                for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float up = row_up(__float_as_uint(most));
+                uint32_t h2[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    h2[i] = half2_bits(__floats2half2_rn(__uint_as_float(w[i] << 16) * (up * sign), __uint_as_float(w[i] & 0xffff0000u) * (up * sign)));
+                *reinterpret_cast<uint4 *>(sq + (row / TC_GROUP_ROWS) * S::Q_BYTES + tc_offset(TC_GROUP_ROWS, row % TC_GROUP_ROWS, x)) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
+                if (x == 0) s_factor[row] = fabsf(p.scale_log2) * pow2_inverse(up);
+            }
+        }
+        fence_async_smem();
+        mbar_arrive(&q_full);
+        const int group = warp >> 2, row = warp * 32 + lane;
+        if (group < n_groups) {
+            const uint32_t t_lane = tmem + ((uint32_t) ((warp & 3) * 32) << 16);
+            const uint32_t t_out = t_lane + S::T_O + group * D;
+            // all warps' rows are in place before the factors are read
+            bool ok = __all_sync(0xffffffffu, wait_suspended(&q_full, 0, &s_abort, p.err));
+            const float factor = s_factor[row];
+            const int seen = reach(min(row, n_rows - 1));
+            float ref = -INFINITY;
+            uint64_t sum2 = 0;    // two zeros
+            for (int i = 0; i < n_tiles && ok; ++i) {
+                const int st = i % NS, b = 2 * group + (i & 1);
+                const uint32_t ph = (i / NS) & 1, b_ph = (i >> 1) & 1;
+                const uint32_t t_s = t_lane + S::T_S + b * KT;
+                // the votes reconverge the warp and make the outcome uniform for the instructions that need all of it
+                bool ready = mbar_try_wait(&s_full[b], b_ph);
+                ready &= mbar_try_wait(&k_full[st], ph);
+                ready &= mbar_try_wait(&v_full[st], ph);
+                if (!__all_sync(0xffffffffu, ready)) {
+                    ok = __all_sync(0xffffffffu, wait_suspended(&s_full[b], b_ph, &s_abort, p.err) && wait_suspended(&k_full[st], ph, &s_abort, p.err) &&
+                                                     wait_suspended(&v_full[st], ph, &s_abort, p.err));
+                    if (!ok) break;
+                }
+                tc_fence_after();
+                const float4 * ks = reinterpret_cast<const float4 *>(k_scale[st]);
+                const float4 * vs = reinterpret_cast<const float4 *>(v_scale[st]);
+                uint32_t s[2][32];
+                tmem_load32(t_s, s[0]);
+                tmem_load32(t_s + 32, s[1]);
+                // the largest of the values' factors that the row may meet here
+                float top = 0.0f, most = -INFINITY;
+                uint64_t on = ~0ull;    // keys that the row sees
+                const bool masked = masked_tile(i, group * TC_GROUP_ROWS) || s_bad[st] == i + 1;
+                if (!masked) {
+                    static_assert(TC_PRODUCER_WARPS == 4, "four maxima");
+                    const float4 x = *reinterpret_cast<const float4 *>(v_top[st]);
+                    top = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
+                } else {
+                    const int key = key0 + i * KT;
+                    on = 0;
+#pragma unroll 4
+                    for (int c = 0; c < KT; ++c)    // a negative factor marks a page that is not there
+                        if (key + c < seen && !(k_scale[st][c] < 0.0f)) {
+                            on |= 1ull << c;
+                            top = fmaxf(top, v_scale[st][c]);
+                        }
+                }
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < KT; c += 4) {
+                    const float4 f = ks[c / 4];
+                    uint32_t * v = s[c / 32] + c % 32;
+                    const float2 x = unpack2(mul2(pack2(__uint_as_float(v[0]), __uint_as_float(v[1])), pack2(f.x, f.y)));
+                    const float2 y = unpack2(mul2(pack2(__uint_as_float(v[2]), __uint_as_float(v[3])), pack2(f.z, f.w)));
+                    v[0] = __float_as_uint(x.x); v[1] = __float_as_uint(x.y); v[2] = __float_as_uint(y.x); v[3] = __float_as_uint(y.y);
+                }
+                if (!masked) {
+                    float part[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+                    for (int c = 0; c < KT; c += 2)
+                        part[c / 2 % 4] = max3(part[c / 2 % 4], __uint_as_float(s[c / 32][c % 32]), __uint_as_float(s[c / 32][c % 32 + 1]));
+                    most = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j] = 0u;
+                    for (int c = 0; c < KT; ++c)
+                        if (on >> c & 1) most = fmaxf(most, __uint_as_float(s[c / 32][c % 32]));
                 }
-                const int d = half * (D / 2) + c;
-                if (there && p.direct) {
-                    float x[16];
+                // weights 2^(s - ref) times a factor stay below 2^7 at a reference that has just risen, and below 2^15 until it rises again
+                const float room = (float) (max((int) (__float_as_uint(top) >> 23), 47) - 127 - 6);
+                const float want = most == -INFINITY ? -INFINITY : most * factor + room;
+                const bool rise = want > ref + 8.0f || (ref == -INFINITY && want > -INFINITY);
+                if (__any_sync(0xffffffffu, rise)) {
+                    const float back = !rise ? 1.0f : ref == -INFINITY ? 0.0f : fast_exp2(ref - want);
+                    if (rise) { sum2 = mul2(sum2, pack2(back, back)); ref = want; }
+                    if (i > 0) {
+                        ok = __all_sync(0xffffffffu, wait_suspended(&pv_done[b ^ 1], ((i - 1) >> 1) & 1, &s_abort, p.err));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 16) {
+                            uint32_t o[16];
+                            tmem_load16(t_out + d, o);
+                            tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) x[j] = sum == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
-                    char * dst = p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head;
-                    float lo[8], hi[8];
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * back);
+                            tmem_store16(t_out + d, o);
+                        }
+                    }
+                }
+                // the weights, over the scores
+                const float base = ref == -INFINITY ? 0.0f : -ref;
+                const uint64_t base2 = pack2(base, base), factor2 = pack2(factor, factor);
+                if (!masked) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) { lo[j] = x[j]; hi[j] = x[8 + j]; }
-                    store8<__nv_bfloat16>(lo, dst, d / 8, p.out_aligned);
-                    store8<__nv_bfloat16>(hi, dst, d / 8 + 1, p.out_aligned);
-                } else if (there) {
-                    float4 * dst = reinterpret_cast<float4 *>(p.part_o + (line * chunks + slot) * D + d);
+                    for (int c = 0; c < KT; c += 4) {
+                        uint32_t * v = s[c / 32] + c % 32;
+                        const float4 g = vs[c / 4];
+                        const float2 x = unpack2(fma2(pack2(__uint_as_float(v[0]), __uint_as_float(v[1])), factor2, base2));
+                        const float2 y = unpack2(fma2(pack2(__uint_as_float(v[2]), __uint_as_float(v[3])), factor2, base2));
+                        const uint64_t u = pack2(fast_exp2(x.x), fast_exp2(x.y)), w = pack2(fast_exp2(y.x), fast_exp2(y.y));
+                        sum2 = add2(sum2, add2(u, w));
+                        const float2 a = unpack2(mul2(u, pack2(g.x, g.y))), d = unpack2(mul2(w, pack2(g.z, g.w)));
+                        s[0][c / 2] = half2_bits(__floats2half2_rn(a.x, a.y));    // over scores that have been used
+                        s[0][c / 2 + 1] = half2_bits(__floats2half2_rn(d.x, d.y));
+                    }
+                } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+                    for (int c = 0; c < KT; c += 2) {
+                        float u[2], v[2];
+#pragma unroll
+                        for (int l = 0; l < 2; ++l) {
+                            const bool see = on >> (c + l) & 1;
+                            u[l] = see ? fast_exp2(fmaf(__uint_as_float(s[(c + l) / 32][(c + l) % 32]), factor, base)) : 0.0f;
+                            v[l] = see ? u[l] * v_scale[st][c + l] : 0.0f;
+                        }
+                        sum2 = add2(sum2, pack2(u[0], u[1]));
+                        s[0][c / 2] = half2_bits(__floats2half2_rn(v[0], v[1]));
+                    }
+                }
+                tmem_store32(t_s, s[0]);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[b]);
+                __syncwarp();
+                if (lane == 0) {    // the tile's factors have been read
+                    mbar_arrive(&k_free[st]);
+                    mbar_arrive(&v_free[st]);
                 }
             }
-            if (there && half == 0) {
-                if (!p.direct) p.part_ml[line * chunks + slot] = make_float2(ref, sum);
-                else if (p.lse) p.lse[line] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
+            // ---- the outputs
+            const int last = n_tiles - 1;
+            if (ok && n_tiles)
+                ok = __all_sync(0xffffffffu, wait_suspended(&pv_done[2 * group + (last & 1)], (last >> 1) & 1, &s_abort, p.err));
+            tc_fence_after();
+            if (ok) {
+                const float2 halves = unpack2(sum2);
+                const float sum = halves.x + halves.y;
+                const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
+                const int64_t line = (int64_t) token * p.n_head + h;
+                const int chunks = p.prefix_chunks + p.own_chunks, slot = PREFIX ? chunk : p.prefix_chunks + chunk;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const bool there = row < n_rows;
+                // 32 by 32 values at a time through the group's query tile, which nothing reads any more, so that a row's values leave together
+                float * stage = reinterpret_cast<float *>(sq + group * S::Q_BYTES + (warp & 3) * 4096);
+                // where the thread's row goes; the warp's threads tell one another
+                const int64_t to = p.direct ? (int64_t) token * p.out_token + (int64_t) h * p.out_head : (line * chunks + slot) * (int64_t) (D * 4);
+                const int in_warp = min(32, n_rows - warp * 32);    // rows of this warp
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    if (n_tiles) {
+                        tmem_load32(t_out + c, o);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = 0u;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        stage[lane * 32 + (j ^ lane)] = !p.direct ? __uint_as_float(o[j]) : sum == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
+                    __syncwarp();
+                    if (!p.direct) {
+#pragma unroll 8
+                        for (int r = 0; r < 32; ++r) {
+                            const int64_t at_row = __shfl_sync(0xffffffffu, to, r);
+                            if (r < in_warp) *reinterpret_cast<float *>(reinterpret_cast<char *>(p.part_o) + at_row + (c + lane) * 4) = stage[r * 32 + (lane ^ r)];
+                        }
+                    } else {
+#pragma unroll 8
+                        for (int r2 = 0; r2 < 32; r2 += 2) {
+                            const int r = r2 + (lane >> 4), d = 2 * (lane & 15);
+                            const int64_t at_row = __shfl_sync(0xffffffffu, to, r);
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(stage[r * 32 + (d ^ r)], stage[r * 32 + ((d + 1) ^ r)]);
+                            char * dst = p.out + at_row + (c + d) * 2;
+                            if (r < in_warp) {
+                                if (p.out_aligned) {
+                                    *reinterpret_cast<__nv_bfloat162 *>(dst) = v;
+                                } else {
+                                    reinterpret_cast<__nv_bfloat16 *>(dst)[0] = v.x;
+                                    reinterpret_cast<__nv_bfloat16 *>(dst)[1] = v.y;
+                                }
+                            }
+                        }
+                    }
+                }
+                if (there) {
+                    if (!p.direct) p.part_ml[line * chunks + slot] = make_float2(ref, sum);
+                    else if (p.lse) p.lse[line] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
+                }
             }
         }
-    } else if (warp < TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS) {
+    } else if (warp < SW + TC_PRODUCER_WARPS) {
         // ------------------------------------------------------------ producers
-        const int q = tid - 32 * TC_SOFTMAX_WARPS, x = q % S::TPR, r0 = q / S::TPR;
+        const int q = tid - 32 * SW, x = q % S::TPR, r0 = q / S::TPR;
         const int32_t * table = PREFIX ? p.prefix_pages : p.pages + (int64_t) seq * p.pages_stride;
         const int shift = p.kv.page_shift, in_page = (1 << shift) - 1, n_pages = (int) (p.kv.n_slots >> shift);
-        int64_t row[S::NL];    // cache row of each pass, -1 behind the last key, -2 where the page is not there
-        auto find = [&](int i) {
+        int slot[S::NL];    // cache slot of each pass, -1 behind the last key, -2 where the page is not there
+        auto find = [&](int part) {    // parts of all tiles, one after the other; all page numbers are fetched together
+            int page[S::NL];
 #pragma unroll
             for (int n = 0; n < S::NL; ++n) {
-                const int key = key0 + i * KT + n * S::ROWS + r0;
-                row[n] = -1;
-                if (key >= key_end) continue;
-                const bool shared = key < front;
-                const int k = shared ? key : key - front;
-                const int page = shared ? p.prefix_pages[k >> shift] : table[k >> shift];
-                if (page < 0 || page >= n_pages) {
-                    report_error(p.err, DEV_ERR_BAD_SLOT);
-                    row[n] = -2;
-                } else {
-                    row[n] = (((int64_t) page * p.kv.n_head + head) << shift) + (k & in_page);
-                }
+                const int key = key0 + (part * S::NL + n) * S::ROWS + r0, k = key < front ? key : key - front;
+                const int32_t * at = (key < front ? p.prefix_pages : table) + (k >> shift);
+                page[n] = key < key_end ? *at : 0;
             }
+            bool bad = false;
+#pragma unroll
+            for (int n = 0; n < S::NL; ++n) {
+                const int key = key0 + (part * S::NL + n) * S::ROWS + r0, k = key < front ? key : key - front;
+                const bool there = page[n] >= 0 && page[n] < n_pages;
+                slot[n] = key >= key_end ? -1 : there ? (page[n] << shift) + (k & in_page) : -2;
+                bad |= slot[n] == -2;
+            }
+            if (bad) report_error(p.err, DEV_ERR_BAD_SLOT);
         };
         TcPiece<TYPE, D> k, v;
-        uint32_t there = 0, gone = 0;    // of the tile whose values are held
-        auto flags = [&]() {
-            there = gone = 0;
-#pragma unroll
-            for (int n = 0; n < S::NL; ++n) {
-                if (row[n] >= 0) there |= 1u << n;
-                if (row[n] == -2) gone |= 1u << n;
-            }
-        };
-        if (n_tiles) {
+        float top = 0.0f;
+        const int n_parts = n_tiles * S::PARTS;
+        if (n_parts) {
             find(0);
-            tc_load<TYPE, D>(k, p.kv.k, p.kv.k_scale, row, x);
-            tc_load<TYPE, D>(v, p.kv.v, p.kv.v_scale, row, x);
+            tc_load<TYPE, D>(k, p.kv.k, p.kv.k_scale, p.kv, slot, head, x);
+            tc_load<TYPE, D>(v, p.kv.v, p.kv.v_scale, p.kv, slot, head, x);
         }
-        for (int i = 0; i < n_tiles; ++i) {
-            const int st = i & 1;
-            const uint32_t ph = (i >> 1) & 1;
-            flags();
-            const bool masked = masked_tile(i);
-            if (!__all_sync(0xffffffffu, wait_or_abort<20>(&k_free[st], ph ^ 1u, &s_abort, p.err))) break;
+        for (int part = 0; part < n_parts; ++part) {
+            const int i = part / S::PARTS, in_tile = part % S::PARTS, st = i % NS;
+            const uint32_t ph = (i / NS) & 1;
+            uint32_t there = 0, gone = 0;
 #pragma unroll
             for (int n = 0; n < S::NL; ++n) {
-                const float f = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, n * S::ROWS + r0, x, there >> n & 1, false);
-                if (x == 0) k_scale[st][n * S::ROWS + r0] = gone >> n & 1 ? -1.0f : there >> n & 1 ? f : 0.0f;
+                if (slot[n] >= 0) there |= 1u << n;
+                if (slot[n] == -2) gone |= 1u << n;
+            }
+            const bool masked = masked_tile(i, 0);
+            const int to = in_tile * S::NL * S::ROWS + r0;
+            if (in_tile == 0 && !__all_sync(0xffffffffu, wait_suspended(&k_free[st], ph ^ 1u, &s_abort, p.err))) break;
+#pragma unroll
+            for (int n = 0; n < S::NL; ++n) {
+                const float f = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, false);
+                if (x == 0) k_scale[st][to + n * S::ROWS] = gone >> n & 1 ? -1.0f : there >> n & 1 ? f : 0.0f;
             }
             if (gone) s_bad[st] = i + 1;
-            fence_async_smem();
-            mbar_arrive(&k_full[st]);
-            if (i + 1 < n_tiles) {
-                find(i + 1);
-                tc_load<TYPE, D>(k, p.kv.k, p.kv.k_scale, row, x);
+            if (in_tile == S::PARTS - 1) {
+                fence_async_smem();
+                mbar_arrive(&k_full[st]);
             }
-            if (!__all_sync(0xffffffffu, wait_or_abort<20>(&v_free[st], ph ^ 1u, &s_abort, p.err))) break;
+            if (part + 1 < n_parts) {
+                find(part + 1);
+                tc_load<TYPE, D>(k, p.kv.k, p.kv.k_scale, p.kv, slot, head, x);
+            }
+            if (in_tile == 0 && !__all_sync(0xffffffffu, wait_suspended(&v_free[st], ph ^ 1u, &s_abort, p.err))) break;
 #pragma unroll
             for (int n = 0; n < S::NL; ++n) {
-                const float f = tc_store<TYPE, D, true>(v, n, sv + st * S::KV_BYTES, n * S::ROWS + r0, x, there >> n & 1, masked);
-                if (x == 0) v_scale[st][n * S::ROWS + r0] = there >> n & 1 ? f : 0.0f;
+                const float f = tc_store<TYPE, D, true>(v, n, sv + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, masked);
+                if (x == 0) v_scale[st][to + n * S::ROWS] = there >> n & 1 ? f : 0.0f;
+                top = fmaxf(top, there >> n & 1 ? f : 0.0f);    // not a number: says nothing here, makes the weight one
             }
-            fence_async_smem();
-            mbar_arrive(&v_full[st]);
-            if (i + 1 < n_tiles) tc_load<TYPE, D>(v, p.kv.v, p.kv.v_scale, row, x);
+            if (in_tile == S::PARTS - 1) {
+                const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));    // factors are not negative: their bits have their order
+                if (lane == 0) v_top[st][warp - SW] = __uint_as_float(most);
+                top = 0.0f;
+                fence_async_smem();
+                mbar_arrive(&v_full[st]);
+            }
+            if (part + 1 < n_parts) tc_load<TYPE, D>(v, p.kv.v, p.kv.v_scale, p.kv, slot, head, x);
         }
     } else if (lane == 0) {
         // ------------------------------------------------------------ products
-        constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t) (KT >> 3) << 17) | ((128u >> 4) << 24);
-        constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | ((uint32_t) (D >> 3) << 17) | ((128u >> 4) << 24);    // second operand: head_dim contiguous
-        auto values = [&](int i) {
-            const int st = i & 1;
-            const uint32_t ph = (i >> 1) & 1;
-            if (!wait_or_abort(&p_full[st], ph, &s_abort, p.err) || !wait_or_abort(&v_full[st], ph, &s_abort, p.err)) return false;
-            tc_fence_after();
-            const uint32_t b = smem_u32(sv + st * S::KV_BYTES);
+        const int g = (warp - SW - TC_PRODUCER_WARPS) >> 1;
+        const bool outputs = (warp - SW - TC_PRODUCER_WARPS) & 1;
+        if (g < n_groups && !outputs) {
+            constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (KT >> 3) << 17) | ((128u >> 4) << 24);
+            const uint32_t a = smem_u32(sq) + g * S::Q_BYTES;
+            const bool queries = wait_suspended(&q_full, 0, &s_abort, p.err);
+            for (int i = 0; i < n_tiles && queries; ++i) {
+                const int st = i % NS, b = 2 * g + (i & 1);
+                // the scores go over the weights of two tiles back
+                if (!wait_suspended(&k_full[st], (i / NS) & 1, &s_abort, p.err) || !wait_suspended(&pv_done[b], ((i >> 1) & 1) ^ 1u, &s_abort, p.err)) break;
+                tc_fence_after();
+                const uint32_t k = smem_u32(sk + st * S::KV_BYTES);
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-                umma_f16_ts(tmem + S::T_O, tmem + S::T_P + st * (KT / 2) + 8 * k, umma_desc_v(b + 2048 * k, KT * 128), IDESC_O, i > 0 || k > 0);
-            umma_commit(&v_free[st]);
-            umma_commit(&pv_done[st]);
-            return true;
-        };
-        bool ok = true;
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const int st = i & 1;
-            const uint32_t ph = (i >> 1) & 1;
-            ok = wait_or_abort(&k_full[st], ph, &s_abort, p.err) && wait_or_abort(&s_free[st], ph ^ 1u, &s_abort, p.err);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t a = smem_u32(sq), b = smem_u32(sk + st * S::KV_BYTES);
+                for (int s = 0; s < D / 16; ++s)
+                    umma_f16(tmem + S::T_S + b * KT, umma_desc_k128(a + (s / 4) * (TC_GROUP_ROWS * 128) + (s % 4) * 32),
+                             umma_desc_k128(k + (s / 4) * (KT * 128) + (s % 4) * 32), IDESC, s > 0);
+                umma_commit(&s_full[b]);
+                umma_commit(&k_free[st]);
+            }
+        } else if (g < n_groups) {
+            constexpr uint32_t IDESC = (1u << 4) | (1u << 16) | ((uint32_t) (D >> 3) << 17) | ((128u >> 4) << 24);    // second operand: head_dim contiguous
+            for (int i = 0; i < n_tiles; ++i) {
+                const int st = i % NS, b = 2 * g + (i & 1);
+                if (!wait_suspended(&v_full[st], (i / NS) & 1, &s_abort, p.err) || !wait_suspended(&p_full[b], (i >> 1) & 1, &s_abort, p.err)) break;
+                tc_fence_after();
+                const uint32_t v = smem_u32(sv + st * S::KV_BYTES);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                umma_f16(tmem + S::T_S + st * KT, umma_desc_k128(a + (k / 4) * (TC_ROWS * 128) + (k % 4) * 32),
-                         umma_desc_k128(b + (k / 4) * (KT * 128) + (k % 4) * 32), IDESC_S, k > 0);
-            umma_commit(&s_full[st]);
-            umma_commit(&k_free[st]);
-            if (i > 0) ok = values(i - 1);
+                for (int s = 0; s < KT / 16; ++s)
+                    umma_f16_ts(tmem + S::T_O + g * D, tmem + S::T_S + b * KT + 8 * s, umma_desc_v(v + 2048 * s, KT * 128), IDESC, i > 0 || s > 0);
+                umma_commit(&pv_done[b]);
+                umma_commit(&v_free[st]);
+            }
         }
-        if (ok && n_tiles) values(n_tiles - 1);
     }
 
-    // ---- teardown: every wait above is bounded; the softmax warps have waited for the last product
+    // ---- teardown: every wait above is bounded; the softmax warps have waited for the last products
     if (s_abort) {
         // products that were issued but not waited for end within microseconds: a bounded grace period
         const uint64_t t0 = global_timer_ns();
@@ -571,7 +707,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attend_tc_kernel(const __grid_c
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == TC_SOFTMAX_WARPS + TC_PRODUCER_WARPS) tmem_dealloc(tmem, 512);
+    if (warp == SW + TC_PRODUCER_WARPS) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace b200moe

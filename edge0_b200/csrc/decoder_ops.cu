@@ -134,16 +134,31 @@ struct AttnPlan {
     size_t part_o, bytes;
 };
 
-// From so many rows to a key/value head the kernels with 128 rows to a tile run (bf16 queries).
+// Up to so many chunks a row is joined by one warp.
+constexpr int JOIN_FEW = 16;
+// From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries).
 constexpr int ATTN_TC_ROWS = 64;
-constexpr int TC_TILE = 16;    // nt of the kernels with 128 rows to a tile
+constexpr int TC_TILE = 0;     // nt of those kernels, whose tile goes by the head_dim
 
 int tile_units(int64_t rows, int most) { return rows <= 8 ? 1 : rows <= 16 ? 2 : most; }
 
 // keys to a chunk, a multiple of `unit`, so that `base` blocks of whole length become about `blocks`
 void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int & chunk, int & chunks) {
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((len + unit - 1) / unit, blocks / std::max<int64_t>(base, 1)));
+    const int64_t n = std::max<int64_t>(1, std::min({ (len + unit - 1) / unit, blocks / std::max<int64_t>(base, 1), (int64_t) JOIN_CHUNKS / 2 }));
     chunk = (int) std::max<int64_t>(unit, ((len + n - 1) / n + unit - 1) / unit * unit);
+    chunks = (int) ((len + chunk - 1) / chunk);
+}
+
+// The same for the kernels with tiles of many rows, one block to an SM: the number of chunks whose waves take least, in tiles of 64 keys.  A block
+// costs about three tiles beside its keys (queries in, outputs out), and the join about four.
+void split_keys_tc(int64_t len, int64_t base, int64_t sms, int & chunk, int & chunks) {
+    const int64_t tiles = std::max<int64_t>(1, (len + 63) / 64);
+    int64_t best = INT64_MAX, n_best = 1;
+    for (int64_t n = 1; n <= std::min<int64_t>(tiles, 64); ++n) {
+        const int64_t cost = (base * n + sms - 1) / sms * ((tiles + n - 1) / n + 3) + (n > 1 ? 4 : 0);
+        if (cost < best) { best = cost; n_best = n; }
+    }
+    chunk = (int) ((tiles + n_best - 1) / n_best * 64);
     chunks = (int) ((len + chunk - 1) / chunk);
 }
 
@@ -162,7 +177,7 @@ int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn
 
 int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int n_head, int n_tokens, bool f32, AttnPlan & pl) {
     const int group = n_head / c->n_head_kv, most = attend_tiles(c->head_dim, f32);
-    const int pass = 32 * ATTN_WARPS, tc_pass = c->head_dim == 256 ? 64 : 128;
+    const int pass = 32 * ATTN_WARPS;
     const int64_t blocks = (int64_t) ctx->sm_count * 6;
     pl = AttnPlan{};
     const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
@@ -170,15 +185,18 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     // sequences that fill tiles of their own walk the prefix themselves: the products take the same time, and nothing is left to join
     if (a->prefix_len && own_tc && own_rows >= 128) pl.own_prefix = a->prefix_len;
     pl.own_nt = own_tc ? TC_TILE : tile_units(own_rows, most);
-    pl.own_tiles = (int) ((own_rows + 8 * pl.own_nt - 1) / (8 * pl.own_nt));
-    split_keys((int64_t) a->max_kv_len + pl.own_prefix, (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, own_tc ? ctx->sm_count : blocks,
-               own_tc ? tc_pass : pass, pl.own_chunk, pl.own_chunks);
+    auto tiles = [&](int64_t n, int nt) { const int tile = nt == TC_TILE ? attend_tc_rows(c->head_dim) : 8 * nt; return (int) ((n + tile - 1) / tile); };
+    pl.own_tiles = tiles(own_rows, pl.own_nt);
+    const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, own_len = (int64_t) a->max_kv_len + pl.own_prefix;
+    if (own_tc) split_keys_tc(own_len, own_base, ctx->sm_count, pl.own_chunk, pl.own_chunks);
+    else split_keys(own_len, own_base, blocks, pass, pl.own_chunk, pl.own_chunks);
     pl.own_chunks = std::max(pl.own_chunks, 1);
     if (a->prefix_len && !pl.own_prefix) {
         pl.prefix_nt = prefix_tc ? TC_TILE : tile_units(rows, most);
-        pl.prefix_tiles = (int) ((rows + 8 * pl.prefix_nt - 1) / (8 * pl.prefix_nt));
-        split_keys(a->prefix_len, (int64_t) c->n_head_kv * pl.prefix_tiles, prefix_tc ? ctx->sm_count : blocks, prefix_tc ? tc_pass : pass, pl.prefix_chunk,
-                   pl.prefix_chunks);
+        pl.prefix_tiles = tiles(rows, pl.prefix_nt);
+        const int64_t base = (int64_t) c->n_head_kv * pl.prefix_tiles;
+        if (prefix_tc) split_keys_tc(a->prefix_len, base, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
+        else split_keys(a->prefix_len, base, blocks, pass, pl.prefix_chunk, pl.prefix_chunks);
     }
     const int64_t limit = (int64_t) 1 << 31;
     if ((int64_t) a->n_seq * c->n_head_kv * pl.own_tiles * pl.own_chunks >= limit || (int64_t) c->n_head_kv * pl.prefix_tiles * pl.prefix_chunks >= limit)
@@ -191,19 +209,24 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     return B200MOE_OK;
 }
 
-template <int D>
-int launch_join(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t st) {
+template <int D, int WARPS>
+int launch_join_w(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t st) {
+    constexpr int LINES = JOIN_THREADS / 32 / WARPS;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) ((int64_t) p.n_tokens * p.n_head));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3((unsigned) (((int64_t) p.n_tokens * p.n_head + LINES - 1) / LINES));
+    cfg.blockDim = dim3(JOIN_THREADS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    CUDA_TRY(ctx, f32 ? cudaLaunchKernelEx(&cfg, attend_join_kernel<D, float>, p) : cudaLaunchKernelEx(&cfg, attend_join_kernel<D, __nv_bfloat16>, p));
+    CUDA_TRY(ctx, f32 ? cudaLaunchKernelEx(&cfg, attend_join_kernel<D, float, WARPS>, p) : cudaLaunchKernelEx(&cfg, attend_join_kernel<D, __nv_bfloat16, WARPS>, p));
     return check_launch(ctx, "attention join");
+}
+template <int D>
+int launch_join(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t st) {
+    return p.prefix_chunks + p.own_chunks <= JOIN_FEW ? launch_join_w<D, 1>(ctx, p, f32, st) : launch_join_w<D, 8>(ctx, p, f32, st);
 }
 
 }  // namespace
