@@ -36,20 +36,10 @@ class Tensor(C.Structure):
     _fields_ = [("data", C.c_void_p), ("ne", C.c_int64 * 4), ("nb", C.c_int64 * 4)]
 
 
-class Rope(C.Structure):
-    _fields_ = [("n_rot", C.c_int32), ("n_axes", C.c_int32), ("sections", C.c_int32 * 4), ("interleaved", C.c_int32), ("adjacent", C.c_int32),
-                ("inverse", C.c_int32), ("reserved_", C.c_int32), ("base", C.c_double)]
-
-
 class KvCacheDesc(C.Structure):
     """b200moe_kv_cache"""
     _fields_ = [(n, C.c_int32) for n in ("type", "n_head_kv", "head_dim", "page_size")] + [("n_pages", C.c_int64)] + [
         (n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")]
-
-
-class Attn(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("n_seq", "max_new", "max_kv_len", "prefix_len", "pages_stride")] + [("scale", C.c_float)] + [
-        (n, C.c_void_p) for n in ("q_start", "kv_len", "pages", "prefix_pages")]
 
 
 class Counters(C.Structure):
@@ -111,13 +101,13 @@ SIGNATURES = {
     "b200moe_op_soft_max": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_float, C.c_void_p]),
     "b200moe_op_argsort_desc": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_void_p]),
     "b200moe_op_mul_mat_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
-    "b200moe_op_rope": (C.c_int, [C.c_void_p, C.POINTER(Tensor), C.c_int, C.c_void_p, C.POINTER(Rope), C.POINTER(Tensor), C.c_void_p]),
+    # descriptions of tensors and calls may be packed bytes here (moe.rows_view, kv_cache.py), which cost a tenth of a ctypes structure to make
+    "b200moe_op_rope": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200moe_kv_cache_bytes": (C.c_int, [C.POINTER(KvCacheDesc), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
-    "b200moe_kv_write": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Tensor), C.POINTER(Tensor), C.c_int, C.c_void_p, C.c_void_p]),
-    "b200moe_kv_read": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.c_void_p, C.POINTER(Tensor), C.POINTER(Tensor), C.c_int, C.c_void_p]),
-    "b200moe_attention_workspace": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Attn), C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
-    "b200moe_attention": (C.c_int, [C.c_void_p, C.POINTER(KvCacheDesc), C.POINTER(Attn), C.POINTER(Tensor), C.c_int, C.POINTER(Tensor), C.c_void_p,
-                                    C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200moe_kv_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "b200moe_kv_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "b200moe_attention_workspace": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "b200moe_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "b200moe_probe_fp4_tile": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200moe_probe_fp4_rate": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]),
     "b200moe_route_noalloc": (C.c_int, [C.c_int, C.POINTER(Layer), C.c_void_p, C.c_int, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,

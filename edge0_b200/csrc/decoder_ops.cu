@@ -70,7 +70,7 @@ int launch_rope(ContextBase * ctx, const RopeParams & p, bool adjacent, bool wid
     constexpr int VP = 16 / sizeof(T);
     // a token's table of turns serves all its heads; a few tokens to a block where there are many, so that every thread has one to work out
     const int half = p.n_rot / 2;
-    const int per_block = std::max(1, std::min({ ROPE_THREADS / half, p.n_tokens / (4 * ctx->sm_count), 8 }));
+    const int per_block = std::max(1, std::min({ ROPE_THREADS / half, (p.n_tokens + 4 * ctx->sm_count - 1) / (4 * ctx->sm_count), 8 }));
     const int blocks = (p.n_tokens + per_block - 1) / per_block;
     const size_t smem = sizeof(float2) * half * per_block;
     if (smem > 48 * 1024) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "n_rot must be at most 12288");

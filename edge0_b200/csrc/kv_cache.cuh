@@ -97,15 +97,37 @@ __device__ __forceinline__ int kv_code(float x, float d, float inv, int top) {
     return max(-top, min(top, code));
 }
 
-// the largest |x| of a group as its bits, which order infinities and NaN behind every number; GROUP threads
+// the largest |x| of a group of GROUP threads; NaN where one is
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 template <int GROUP>
-__device__ __forceinline__ uint32_t group_amax(const float (&x)[8]) {
-    uint32_t m = 0;
+__device__ __forceinline__ float group_amax(const float (&x)[8]) {
+    float m = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) m = max_or_nan(m, fabsf(x[j]));
 #pragma unroll
-    for (int o = GROUP / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = GROUP / 2; o > 0; o >>= 1) m = max_or_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
+}
+
+// Codes of eight values as offset + code in the low bits of each word.  Adding 1.5 * 2^23 rounds the product with the reciprocal to a whole number in
+// the sum's low bits; the remainders say whether one of the eight lies on or over a border, which is settled one by one.  d >= 2^-120: no
+// product leaves the normal range, and none is rounded above the largest code.
+__device__ __forceinline__ void kv_codes(uint32_t (&code)[8], const float (&x)[8], float d, int top, int offset) {
+    const float magic = 12582912.0f + (float) offset, inv = __frcp_rn(d);
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = __fmaf_rn(x[j], inv, magic);
+        most = fmaxf(most, fabsf(__fmaf_rn(-(t - magic), d, x[j])));
+        code[j] = __float_as_uint(t);
+    }
+    if (most + most >= d)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) code[j] = (uint32_t) (offset + kv_code(x[j], d, inv, top));
 }
 
 template <int TYPE, int D, bool VALUES>
@@ -115,26 +137,23 @@ __device__ __forceinline__ void kv_store_row(const float (&x)[8], uint8_t * rows
         if (on) store8<__nv_bfloat16>(x, reinterpret_cast<char *>(at), i, 1);
         return;
     }
-    constexpr int TOP = TYPE == KV_Q8 ? 127 : 7;
-    const uint32_t bits = group_amax<TYPE == KV_Q8 ? D / 8 : 4>(x);
-    float d = bits < 0x7f800000u ? __fdiv_rn(__uint_as_float(bits), (float) TOP) : __uint_as_float(0x7fffffffu);
+    constexpr int TOP = TYPE == KV_Q8 ? 127 : 7, OFFSET = TOP + 1;
+    const float most = group_amax<TYPE == KV_Q8 ? D / 8 : 4>(x);
+    float d = most < INFINITY ? __fdiv_rn(most, (float) TOP) : __uint_as_float(0x7fffffffu);
     if (TYPE == KV_Q4) d = __bfloat162float(__float2bfloat16_rn(d));
-    int code[8];
-    // below 2^-120 the reciprocal, or a product with it, may leave the normal range: divide
-    const float inv = d >= 0x1p-120f ? __frcp_rn(d) : 0.0f;
+    uint32_t code[8];
+    if (d >= 0x1p-120f) {
+        kv_codes(code, x, d, TOP, OFFSET);
+    } else {    // nothing but zeros, something that cannot be quantised, or values so small that quotients are taken in double
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        code[j] = 0;
-        if (inv > 0.0f) code[j] = kv_code(x[j], d, inv, TOP);
-        else if (d > 0.0f) code[j] = max(-TOP, min(TOP, (int) rint((double) x[j] / (double) d)));
+        for (int j = 0; j < 8; ++j) code[j] = (uint32_t) (OFFSET + (d > 0.0f ? max(-TOP, min(TOP, (int) rint((double) x[j] / (double) d))) : 0));
     }
     if (!on) return;
     if (TYPE == KV_Q8) {
         uint32_t w[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
-            w[j] = (uint32_t) (code[4 * j] + 128) | (uint32_t) (code[4 * j + 1] + 128) << 8 | (uint32_t) (code[4 * j + 2] + 128) << 16 |
-                   (uint32_t) (code[4 * j + 3] + 128) << 24;
+            w[j] = __byte_perm(__byte_perm(code[4 * j], code[4 * j + 1], 0x0040), __byte_perm(code[4 * j + 2], code[4 * j + 3], 0x0040), 0x5410);
         *reinterpret_cast<uint2 *>(at + 8 * i) = make_uint2(w[0], w[1]);
         if (i == 0) static_cast<float *>(scales)[row] = d;
     } else {
@@ -142,7 +161,7 @@ __device__ __forceinline__ void kv_store_row(const float (&x)[8], uint8_t * rows
         const int g = i / 4, c = i % 4, run = g / GB, gr = g % GB;
         uint32_t w = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w |= (uint32_t) (code[j] + 8) << (4 * j);
+        for (int j = 0; j < 8; ++j) w |= (code[j] & 15u) << (4 * j);
         uint8_t * p = at + run * 16 * GB;
         if (VALUES) {
             *reinterpret_cast<uint16_t *>(p + 2 * ((2 * c) * GB + gr)) = (uint16_t) w;

@@ -55,70 +55,82 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N) Pack { T v[N]; };
 
 constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_ITEMS = 4;    // items of a thread whose loads are in flight together
+constexpr int ROPE_ROWS = 2;    // heads of a thread whose loads are in flight together: with four, the registers leave two blocks to an SM
 
-// VP pairs to an item: 16 bytes of either half of a pair, or 1 where that is not aligned
+// VP pairs to a piece: 16 bytes of either half of a pair, or 1 where that is not aligned.  A thread keeps its piece of the head and walks the
+// heads of the block's tokens.
 template <typename T, int VP, bool ADJACENT>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const RopeParams p, int tokens_per_block) {
-    extern __shared__ float2 turn[];    // [tokens_per_block][n_rot / 2]
+__global__ void __launch_bounds__(ROPE_THREADS, 4) rope_kernel(const __grid_constant__ RopeParams p, int tokens_per_block) {
+    extern __shared__ float2 turn[];    // [tokens_per_block][VP][n_rot / 2 / VP]: neighbouring pieces read neighbouring words
     typedef Pack<T, VP> V;
     const int half = p.n_rot / 2;
     const int t0 = blockIdx.x * tokens_per_block, nt = min(tokens_per_block, p.n_tokens - t0);
-    for (int e = threadIdx.x; e < nt * half; e += ROPE_THREADS) {
-        const int t = e / half, i = e - t * half;
-        const double pos = (double) p.pos[(int64_t) rope_axis(p, i) * p.n_tokens + t0 + t];
-        double r = pos * exp2((double) i * p.log2_step - p.log2_turn);
-        r -= rint(r);
-        float s, c;
-        sincospif(2.0f * (float) r, &s, &c);
-        turn[e] = make_float2(c, p.sign * s);
-    }
-    __syncthreads();
+    const int pieces = half / VP + (p.copy_rest ? (p.head_dim - p.n_rot) / (2 * VP) : 0);    // of a head
+    const int width = min(pieces, ROPE_THREADS), per_pass = ROPE_THREADS / width;              // heads to a pass of the block
+    const int sub = threadIdx.x / width;
 
-    const int turned = half / VP, rest = p.copy_rest ? (p.head_dim - p.n_rot) / (2 * VP) : 0;
-    const int per_head = turned + rest, per_token = per_head * p.n_head;
-    for (int base = threadIdx.x; base < nt * per_token; base += ROPE_THREADS * ROPE_ITEMS) {
-        V a[ROPE_ITEMS], b[ROPE_ITEMS];
+    for (int piece = threadIdx.x - sub * width, begun = 0; piece < pieces || !begun; piece += ROPE_THREADS) {
+        const bool on = sub < per_pass && piece < pieces;
+        const int i = piece * VP;
+        // behind the turned pairs: 2 VP values at n_rot + 2 (i - half), as for pairs of neighbours
+        const bool flat = ADJACENT || i >= half;
+        const int64_t at_a = (flat ? 2 * i : i) * (int64_t) sizeof(T), at_b = (flat ? 2 * i + VP : i + half) * (int64_t) sizeof(T);
+        int t = sub / p.n_head, h = sub - t * p.n_head;
+        for (bool more = true; more || !begun;) {
+            V a[ROPE_ROWS], b[ROPE_ROWS];
+            int tt[ROPE_ROWS], hh[ROPE_ROWS];
 #pragma unroll
-        for (int u = 0; u < ROPE_ITEMS; ++u) {
-            const int e = base + u * ROPE_THREADS;
-            if (e >= nt * per_token) break;
-            const int t = e / per_token, q = e - t * per_token, h = q / per_head, i = (q - h * per_head) * VP;
-            const T * row = reinterpret_cast<const T *>(p.x + (int64_t) (t0 + t) * p.x_token + (int64_t) h * p.x_head);
-            // behind the turned pairs: 2 VP values at n_rot + 2 (i - half), as for pairs of neighbours
-            const bool flat = ADJACENT || i >= half;
-            a[u] = *reinterpret_cast<const V *>(row + (flat ? 2 * i : i));
-            b[u] = *reinterpret_cast<const V *>(row + (flat ? 2 * i + VP : i + half));
-        }
+            for (int u = 0; u < ROPE_ROWS; ++u) {
+                tt[u] = on && t < nt ? t : -1;
+                hh[u] = h;
+                if (tt[u] >= 0) {
+                    const char * row = p.x + (int64_t) (t0 + t) * p.x_token + (int64_t) h * p.x_head;
+                    a[u] = *reinterpret_cast<const V *>(row + at_a);
+                    b[u] = *reinterpret_cast<const V *>(row + at_b);
+                }
+                for (h += per_pass; h >= p.n_head; h -= p.n_head) ++t;
+            }
+            more = on && t < nt;
+            if (!begun) {    // the turns, while the first rows are on their way
+                begun = 1;
+                for (int e = threadIdx.x; e < nt * half; e += ROPE_THREADS) {
+                    const int te = e / half, ie = e - te * half;
+                    const double pos = (double) p.pos[(int64_t) rope_axis(p, ie) * p.n_tokens + t0 + te];
+                    double r = pos * exp2((double) ie * p.log2_step - p.log2_turn);
+                    r -= rint(r);
+                    float s, c;
+                    sincospif(2.0f * (float) r, &s, &c);
+                    turn[te * half + ie % VP * (half / VP) + ie / VP] = make_float2(c, p.sign * s);
+                }
+                __syncthreads();
+            }
 #pragma unroll
-        for (int u = 0; u < ROPE_ITEMS; ++u) {
-            const int e = base + u * ROPE_THREADS;
-            if (e >= nt * per_token) break;
-            const int t = e / per_token, q = e - t * per_token, h = q / per_head, i = (q - h * per_head) * VP;
-            T * row = reinterpret_cast<T *>(p.dst + (int64_t) (t0 + t) * p.dst_token + (int64_t) h * p.dst_head);
-            const bool flat = ADJACENT || i >= half;
-            V c = a[u], d = b[u];
-            if (i < half) {
+            for (int u = 0; u < ROPE_ROWS; ++u) {
+                if (tt[u] < 0) continue;
+                V c = a[u], d = b[u];
+                if (i < half) {
 #pragma unroll
-                for (int j = 0; j < VP; ++j) {
-                    const float2 w = turn[t * half + i + j];
-                    if (ADJACENT) {    // pair j is values 2j, 2j + 1 of the 2 VP
-                        const float x0 = to_float(2 * j < VP ? a[u].v[(2 * j) % VP] : b[u].v[(2 * j) % VP]);
-                        const float x1 = to_float(2 * j + 1 < VP ? a[u].v[(2 * j + 1) % VP] : b[u].v[(2 * j + 1) % VP]);
-                        const T y0 = from_float<T>(x0 * w.x - x1 * w.y), y1 = from_float<T>(x0 * w.y + x1 * w.x);
-                        if (2 * j < VP) c.v[(2 * j) % VP] = y0;
-                        else d.v[(2 * j) % VP] = y0;
-                        if (2 * j + 1 < VP) c.v[(2 * j + 1) % VP] = y1;
-                        else d.v[(2 * j + 1) % VP] = y1;
-                    } else {
-                        const float x0 = to_float(a[u].v[j]), x1 = to_float(b[u].v[j]);
-                        c.v[j] = from_float<T>(x0 * w.x - x1 * w.y);
-                        d.v[j] = from_float<T>(x0 * w.y + x1 * w.x);
+                    for (int j = 0; j < VP; ++j) {
+                        const float2 w = turn[tt[u] * half + j * (half / VP) + piece];
+                        if (ADJACENT) {    // pair j is values 2j, 2j + 1 of the 2 VP
+                            const float x0 = to_float(2 * j < VP ? a[u].v[(2 * j) % VP] : b[u].v[(2 * j) % VP]);
+                            const float x1 = to_float(2 * j + 1 < VP ? a[u].v[(2 * j + 1) % VP] : b[u].v[(2 * j + 1) % VP]);
+                            const T y0 = from_float<T>(x0 * w.x - x1 * w.y), y1 = from_float<T>(x0 * w.y + x1 * w.x);
+                            if (2 * j < VP) c.v[(2 * j) % VP] = y0;
+                            else d.v[(2 * j) % VP] = y0;
+                            if (2 * j + 1 < VP) c.v[(2 * j + 1) % VP] = y1;
+                            else d.v[(2 * j + 1) % VP] = y1;
+                        } else {
+                            const float x0 = to_float(a[u].v[j]), x1 = to_float(b[u].v[j]);
+                            c.v[j] = from_float<T>(x0 * w.x - x1 * w.y);
+                            d.v[j] = from_float<T>(x0 * w.y + x1 * w.x);
+                        }
                     }
                 }
+                char * row = p.dst + (int64_t) (t0 + tt[u]) * p.dst_token + (int64_t) hh[u] * p.dst_head;
+                *reinterpret_cast<V *>(row + at_a) = c;
+                *reinterpret_cast<V *>(row + at_b) = d;
             }
-            *reinterpret_cast<V *>(row + (flat ? 2 * i : i)) = c;
-            *reinterpret_cast<V *>(row + (flat ? 2 * i + VP : i + half)) = d;
         }
     }
 }

@@ -8,13 +8,15 @@ libedge0_b200.so.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
 
-from .capi import KV_BF16, KV_Q4, KV_Q8, Attn, KvCacheDesc
-from .moe import Context, _ptr, _x_type, int32_on, rows_view
+from .capi import KV_BF16, KV_Q4, KV_Q8, KvCacheDesc
+from .moe import Context, _x_type, int32_on, rows_view
 
+_pack_attn = struct.Struct("=5if4q").pack
 KIND_BY_NAME = {"bf16": KV_BF16, "q8": KV_Q8, "q4": KV_Q4}
 
 
@@ -38,37 +40,35 @@ class KvCache:
         for name in ("k", "v", "k_scale", "v_scale"):
             t = getattr(self, name)
             setattr(self.desc, name, None if t is None else t.data_ptr())
+        self._desc = bytes(self.desc)
+        self._need = {}    # bytes of workspace by the sizes of a call
 
     def nbytes(self) -> int:
         return sum(t.numel() for t in (self.k, self.v, self.k_scale, self.v_scale) if t is not None)
 
-    def _here(self, t: torch.Tensor, what: str) -> torch.Tensor:
-        if t.device != self.device:
-            raise ValueError(f"{what} must be on {self.device}")
-        return t
-
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """k, v [T, n_head_kv, head_dim] float32 or bfloat16 go to slots int32 [T]; slots below zero are passed over, the others must differ."""
+        c = self.ctx
+        dev = c.device
         if k.dtype != v.dtype:
             raise TypeError("k and v must have the same type")
-        s = int32_on(slots, self.device, "slots", (k.shape[0],))
-        c = self.ctx
-        c.check(c.lib.b200moe_kv_write(c.handle, C.byref(self.desc), C.byref(rows_view(self._here(k, "k"), "k")), C.byref(rows_view(self._here(v, "v"), "v")),
-                                       _x_type(k), s, c._stream()))
+        s = int32_on(slots, dev, "slots", k.shape[:1])
+        c.check(c.lib.b200moe_kv_write(c.handle, self._desc, rows_view(k, dev, "k"), rows_view(v, dev, "v"), _x_type(k), s, c._stream()))
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16, out=None):
         """The (k, v) that slots int32 [T] hold, [T, n_head_kv, head_dim] each; slots below zero give zeros.  out: that pair, allocated by the caller."""
-        s = int32_on(slots, self.device, "slots", (slots.numel(),))
+        c = self.ctx
+        dev = c.device
+        n = slots.numel()
+        s = int32_on(slots, dev, "slots", (n,))
         if out is None:
-            shape = (slots.numel(), self.n_head_kv, self.head_dim)
-            k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            shape = (n, self.n_head_kv, self.head_dim)
+            k, v = slots.new_empty(shape, dtype=dtype), slots.new_empty(shape, dtype=dtype)
         else:
             k, v = out
-            if k.dtype != v.dtype or k.shape[0] != slots.numel():
+            if k.dtype != v.dtype or k.shape[0] != n:
                 raise ValueError("out must be a pair of [T, n_head_kv, head_dim] tensors of one type")
-        c = self.ctx
-        c.check(c.lib.b200moe_kv_read(c.handle, C.byref(self.desc), s, C.byref(rows_view(self._here(k, "k"), "k")), C.byref(rows_view(self._here(v, "v"), "v")),
-                                      _x_type(k), c._stream()))
+        c.check(c.lib.b200moe_kv_read(c.handle, self._desc, s, rows_view(k, dev, "k"), rows_view(v, dev, "v"), _x_type(k), c._stream()))
         return k, v
 
     def attend(self, q: torch.Tensor, kv_len: torch.Tensor, pages: torch.Tensor, *, max_kv_len: Optional[int] = None,
@@ -82,33 +82,38 @@ class KvCache:
         max_new the most rows of one.  max_kv_len (default: what the table has room for) bounds the lengths; the work is split by it, so a
         near bound is faster than a far one.  scale: default head_dim ** -0.5.  lse float32 [T, n_head] receives the logarithms of the sums.
         out, lse: rows that belong to no sequence stay as they are (a new `out` has zeros there)."""
-        n_seq = kv_len.numel()
-        T, n_head, d = self._here(q, "q").shape
-        a = Attn(n_seq=n_seq, max_new=max_new, prefix_len=prefix_len, scale=d ** -0.5 if scale is None else scale)
-        a.kv_len = int32_on(kv_len, self.device, "kv_len", (n_seq,))
-        a.pages = int32_on(pages, self.device, "pages", (n_seq, pages.shape[-1]))
-        a.pages_stride = pages.shape[-1]
-        a.max_kv_len = a.pages_stride * self.page_size if max_kv_len is None else max_kv_len
-        if q_start is not None:
-            a.q_start = int32_on(q_start, self.device, "q_start", (n_seq + 1,))
-        if prefix_len:
-            if prefix_pages is None or prefix_pages.numel() * self.page_size < prefix_len:
-                raise ValueError(f"prefix_pages must name {-(-prefix_len // self.page_size)} pages")
-            a.prefix_pages = int32_on(prefix_pages, self.device, "prefix_pages", (prefix_pages.numel(),))
-        if out is None:
-            out = (torch.empty if q_start is None and T == n_seq else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
-        elif out.dtype != q.dtype or out.shape != q.shape or out.device != self.device:
-            raise ValueError("out must be like q")
-        if lse is not None and (lse.dtype != torch.float32 or lse.device != self.device or tuple(lse.shape) != (T, n_head) or not lse.is_contiguous()):
-            raise ValueError("lse must be a contiguous float32 [T, n_head] tensor")
         c = self.ctx
-        need = C.c_size_t()
-        c.check(c.lib.b200moe_attention_workspace(c.handle, C.byref(self.desc), C.byref(a), n_head, T, C.byref(need)))
+        dev = c.device
+        n_seq = kv_len.numel()
+        rows = rows_view(q, dev, "q")
+        T, n_head, d = q.shape
+        m = pages.shape[-1]
+        if prefix_len and (prefix_pages is None or prefix_pages.numel() * self.page_size < prefix_len):
+            raise ValueError(f"prefix_pages must name {-(-prefix_len // self.page_size)} pages")
+        bound = m * self.page_size if max_kv_len is None else max_kv_len
+        a = _pack_attn(n_seq, max_new, bound, prefix_len, m, d ** -0.5 if scale is None else scale,
+                       0 if q_start is None else int32_on(q_start, dev, "q_start", (n_seq + 1,)), int32_on(kv_len, dev, "kv_len", (n_seq,)),
+                       int32_on(pages, dev, "pages", (n_seq, m)), int32_on(prefix_pages, dev, "prefix_pages") if prefix_len else 0)
+        if out is None:
+            out = (torch.empty_like if q_start is None and T == n_seq else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+        elif out.dtype != q.dtype or out.shape != q.shape:
+            raise ValueError("out must be like q")
+        if lse is not None and (lse.dtype != torch.float32 or lse.get_device() != dev or tuple(lse.shape) != (T, n_head) or not lse.is_contiguous()):
+            raise ValueError("lse must be a contiguous float32 [T, n_head] tensor")
+        sizes = (n_seq, max_new, bound, prefix_len, m, n_head, T)
+        need = self._need.get(sizes)
+        if need is None:
+            size = C.c_size_t()
+            c.check(c.lib.b200moe_attention_workspace(c.handle, self._desc, a, n_head, T, C.byref(size)))
+            if len(self._need) >= 256:
+                self._need.clear()
+            need = self._need[sizes] = size.value
         if workspace is None:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        elif workspace.device != self.device or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
-        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        c.check(c.lib.b200moe_attention(c.handle, C.byref(self.desc), C.byref(a), C.byref(rows_view(q, "q")), _x_type(q), C.byref(rows_view(out, "out")),
-                                        _ptr(lse), _ptr(workspace), size, c._stream()))
+            workspace = q.new_empty(need, dtype=torch.uint8) if need else None
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev}")
+        else:
+            need = workspace.numel() * workspace.element_size()
+        c.check(c.lib.b200moe_attention(c.handle, self._desc, a, rows, _x_type(q), rows_view(out, dev, "out"), None if lse is None else lse.data_ptr(),
+                                        None if workspace is None else workspace.data_ptr(), need, c._stream()))
         return out

@@ -9,6 +9,7 @@ reverse of ggml's ne[] order: x [T, n_embd], ids [T, k], expert tensors [n_exper
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -16,7 +17,7 @@ import numpy as np
 import torch
 
 from . import capi
-from .capi import TYPE_BF16, TYPE_F32, TYPE_NVFP4, TYPE_Q3_K, B200MoeError, Layer, Observe, Rope, Tensor
+from .capi import TYPE_BF16, TYPE_F32, TYPE_NVFP4, TYPE_Q3_K, B200MoeError, Layer, Observe
 
 TYPE_BY_NAME = {"q3_k": TYPE_Q3_K, "nvfp4": TYPE_NVFP4}
 
@@ -61,25 +62,27 @@ def _x_type(x: torch.Tensor) -> int:
     raise TypeError("activations must be float32 or bfloat16")
 
 
-def rows_view(t: torch.Tensor, what: str) -> Tensor:
-    """b200moe_tensor of rows [T, heads, head_dim] (any strides between tokens and heads; the values of a row side by side)."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] != 1):
-        raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous rows, not {tuple(t.shape)} with strides {t.stride()}")
-    n, h, d = t.shape
+_pack_tensor, _pack_rope = struct.Struct("=9q").pack, struct.Struct("=10id").pack
+
+
+def rows_view(t: torch.Tensor, device: int, what: str) -> bytes:
+    """b200moe_tensor of rows [T, heads, head_dim] on CUDA device `device` (any strides between tokens and heads; the values of a row side by side)."""
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be on cuda:{device}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous rows, not {tuple(shape)} with strides {stride}")
     es = t.element_size()
-    v = Tensor(t.data_ptr())
-    v.ne[:] = (d, h, n, 1)
-    v.nb[:] = (es, t.stride(1) * es, t.stride(0) * es, 0)
-    return v
+    return _pack_tensor(t.data_ptr(), shape[2], shape[1], shape[0], 1, es, stride[1] * es, stride[0] * es, 0)
 
 
-def int32_on(t: torch.Tensor, device: torch.device, what: str, shape=None) -> C.c_void_p:
-    """Pointer of a contiguous int32 tensor on `device` (of `shape`, where given)."""
-    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor on {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+def int32_on(t: torch.Tensor, device: int, what: str, shape=None) -> int:
+    """Address of a contiguous int32 tensor on CUDA device `device` (of `shape`, where given)."""
+    if t.dtype is not torch.int32 or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor on cuda:{device}")
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
-    return C.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def unpack_expert_blobs_nvfp4(blobs: np.ndarray, n_embd: int, n_ff: int, device=None):
@@ -208,7 +211,7 @@ class Context:
         self.check(self.lib.b200moe_synchronize(self.handle, self._stream()))
 
     def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return torch._C._cuda_getCurrentRawStream(self.device)    # current_stream(self.device).cuda_stream without the object around it
 
     def launches(self) -> int:
         c = capi.Counters()
@@ -257,20 +260,18 @@ class Context:
              adjacent: bool = False, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Rotary positions (b200moe_op_rope): x [T, heads, head_dim] float32 or bfloat16, any strides between tokens and heads; pos int32 [T], or
         [axes, T] with `sections` pairs to each axis.  inverse: the way back, also for gradients.  out may be x itself."""
-        device = torch.device("cuda", self.device)
-        if x.device != device:
-            raise ValueError(f"x must be on {device}")
-        T, _, d = x.shape
+        device, shape = self.device, x.shape
+        view = rows_view(x, device, "x")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=device)
-        elif out.dtype != x.dtype or out.device != device or out.shape != x.shape:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        elif out.dtype != x.dtype or out.shape != shape:
             raise ValueError("out must be like x")
-        r = Rope(n_rot=d if n_rot is None else n_rot, interleaved=interleaved, adjacent=adjacent, inverse=inverse, base=base)
-        sections = [r.n_rot // 2] if sections is None else list(sections)
-        r.n_axes = len(sections)
-        r.sections[:len(sections[:4])] = sections[:4]
-        p = int32_on(pos, device, "pos", (T,) if len(sections) == 1 and pos.dim() == 1 else (len(sections), T))
-        self.check(self.lib.b200moe_op_rope(self.handle, C.byref(rows_view(x, "x")), _x_type(x), p, C.byref(r), C.byref(rows_view(out, "out")), self._stream()))
+        n_rot = shape[2] if n_rot is None else n_rot
+        axes = (n_rot // 2,) if sections is None else tuple(sections)
+        n_axes = len(axes)
+        at = int32_on(pos, device, "pos", shape[:1] if n_axes == 1 and pos.dim() == 1 else (n_axes, shape[0]))
+        r = _pack_rope(n_rot, n_axes, *(axes + (0, 0, 0, 0))[:4], interleaved, adjacent, inverse, 0, base)
+        self.check(self.lib.b200moe_op_rope(self.handle, view, _x_type(x), at, r, rows_view(out, device, "out"), self._stream()))
         return out
 
     # ---- expert-parallel exchange (b200moe_ep_*): outputs may be passed in so a step allocates nothing
