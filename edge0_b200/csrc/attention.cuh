@@ -15,14 +15,16 @@
 //   the same, so a lane's pieces are contiguous.  Values: it holds keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them by byte permutes.
 //
 // Precision.  The codes are whole numbers and go into the product exactly; the scales stay outside in fp32: a key's multiplies the score,
-// a value's the weight p.  Q8: codes as f16 (a byte under the exponent of 1024), queries as f16 with a power of two to a row that puts its
-// largest value at 2^14 (bf16 queries lose nothing that is above 2^-28 of the row's largest; fp32 ones are split in two), weights times scales as f16
-// under a power of two that follows the largest scale seen.  Q4 and BF16: bf16 operands; fp32 queries and weights are split in three.
+// a value's the weight p.  Q8 and Q4: codes as f16 (a byte or nibble under the exponent of 1024), queries as f16 with a power of two to a row that
+// puts its largest value at 2^14 (bf16 queries lose nothing that is above 2^-28 of the row's largest; fp32 ones are split in two), weights times scales
+// as f16 under a power of two that follows the largest scale seen.  BF16: bf16 operands; fp32 queries and weights are split in three.
 // For bf16 queries the weights are one f16 (2^-11 of each) or two bf16 (2^-16).  Scores, maxima, sums and outputs are fp32; as the
 // instruction's accumulator drops what falls below its last bit, fp32 queries add its short runs up in fp32 proper.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "context.cuh"
@@ -128,11 +130,14 @@ __device__ __forceinline__ uint32_t bytes_to_half2(uint32_t w, uint32_t sel) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t *>(&r);
 }
-// the low nibbles of w's two 16-bit halves as the bf16 pair n - 8
-__device__ __forceinline__ uint32_t nibbles_to_bf162(uint32_t w) {
-    const uint32_t h = (w & 0x000f000fu) | 0x43004300u;     // 128 + n
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&h), __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308)));
-    return *reinterpret_cast<const uint32_t *>(&r);
+// nibbles 0 and 4, then 1 and 5, of w as the f16 pairs n - 8: 1024 + n less 1032, and (1024 + 16 n) / 16 less 72, both exact
+__device__ __forceinline__ void nibbles_to_half2(uint32_t w, uint32_t & even, uint32_t & odd) {
+    const uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408)));
+    const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&b), __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00)),
+                              __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480)));
+    even = *reinterpret_cast<const uint32_t *>(&x);
+    odd = *reinterpret_cast<const uint32_t *>(&y);
 }
 
 // The lane's share of a 16-key tile, as loaded; and what the products take from it.  KW, VW: 32-bit words of a key's row that a lane holds.
@@ -240,9 +245,7 @@ __device__ __forceinline__ void key_operand(uint32_t (&a)[4], const KeyRegs<TYPE
             a[i] = bytes_to_half2(t.w[i][step], 0x4140);
             a[2 + i] = bytes_to_half2(t.w[i][step], 0x4342);
         } else {
-            const uint32_t w = t.w[i][step / 2] >> (step & 1 ? 8 : 0);
-            a[i] = nibbles_to_bf162(w);
-            a[2 + i] = nibbles_to_bf162(w >> 4);
+            nibbles_to_half2(t.w[i][step / 2] >> (step & 1 ? 8 : 0), a[i], a[2 + i]);
         }
     }
 }
@@ -260,9 +263,8 @@ __device__ __forceinline__ void value_operand(uint32_t (&a)[4], const ValueRegs<
             a[2 * i] = bytes_to_half2(w, 0x4140);
             a[2 * i + 1] = bytes_to_half2(w, 0x4342);
         } else {
-            const uint32_t w = __byte_perm(t.w[2 * i][tile / 4], t.w[2 * i + 1][tile / 4], tile & 2 ? 0x7632 : 0x5410) >> (tile & 1 ? 8 : 0);
-            a[2 * i] = nibbles_to_bf162(w);
-            a[2 * i + 1] = nibbles_to_bf162(w >> 4);
+            const uint32_t w = __byte_perm(t.w[2 * i][tile / 4], t.w[2 * i + 1][tile / 4], tile & 2 ? 0x7632 : 0x5410);
+            nibbles_to_half2(w >> (tile & 1 ? 8 : 0), a[2 * i], a[2 * i + 1]);
         }
     }
 }
@@ -272,16 +274,21 @@ __device__ __forceinline__ int value_dim(int tile, int r) {
     return 64 * (tile / 4) + 8 * r + 2 * (tile & 3);
 }
 
+#ifndef ATTN_KS
+#define ATTN_KS 2
+#define ATTN_MB 3
+#endif
 constexpr int ATTN_WARPS = 4;
 
 template <int TYPE, int D, typename XT, int NT>
 struct AttnShape {
     static constexpr bool F32 = sizeof(XT) == 4;
-    static constexpr bool BF = TYPE != KV_Q8;                                      // operands in bf16, else f16
+    static constexpr bool BF = TYPE == KV_BF16;                                    // operands in bf16, else f16
     static constexpr int QT = F32 ? (BF ? 3 : 2) : 1;                              // terms of a query
     static constexpr int PT = F32 ? (BF ? 3 : 2) : (BF ? 2 : 1);                   // terms of a weight
     static constexpr int STEPS = D / 16;                                           // k steps of the scores, m tiles of the outputs
-    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? 2 : 1;    // 16-key tiles to a pass of a warp
+    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? ATTN_KS : 1;    // 16-key tiles to a pass of a warp
+    static constexpr int MIN_BLOCKS = D <= 128 && NT == 1 && !F32 ? ATTN_MB : 1;
     static constexpr int ROWS = 8 * NT;
     static constexpr int Q_WORDS = QT * STEPS * NT * 64;
     static constexpr size_t SMEM_Q = Q_WORDS * 4 + ROWS * 8;                       // operands, then factor and reach of every row
@@ -291,7 +298,7 @@ struct AttnShape {
 
 // PREFIX: rows are those of the whole batch and keys the prefix's; else blocks belong to a sequence
 template <int TYPE, int D, typename XT, int NT, bool PREFIX>
-__global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::MIN_BLOCKS)) attend_kernel(const __grid_constant__ AttnParams p) {
     typedef AttnShape<TYPE, D, XT, NT> S;
     typedef AttnTile<TYPE, D> A;
     extern __shared__ __align__(16) uint32_t smem[];
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
         }
 
     float o[S::STEPS][NT][4], m[NT][2], l[NT][2];
-    int top[NT][2];    // Q8: exponent bits of the largest value scale that the row has seen, 2^-100 at least
+    int top[NT][2];    // not BF16: exponent bits of the largest value scale that the row has seen, 2^-100 at least
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -495,9 +502,10 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
                 load_keys<TYPE, D>(kr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
             }
         }
-        // ---- softmax
-        bool on[S::KS][NT][4];
-        if (masked) {
+        // ---- softmax and outputs; the form for tiles that some row does not see in full costs a third more
+        auto weigh = [&](auto form) {
+            constexpr bool MASKED = decltype(form)::value;
+            bool on[S::KS][NT][4];
 #pragma unroll
             for (int j = 0; j < S::KS; ++j)
 #pragma unroll
@@ -505,152 +513,170 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int k = key + 16 * j + r + 8 * (i >> 1);
-                        on[j][n][i] = was_good[j] && k < key_end && k < seen[n][i & 1];
+                        on[j][n][i] = !MASKED || (was_good[j] && k < key_end && k < seen[n][i & 1]);
                         s[j][n][i] = on[j][n][i] ? s[j][n][i] * factor[n][i & 1] : -INFINITY;
                     }
-        } else {
+            // the largest scale of each key's values; NaN scales say nothing here, they make the weight NaN
+            float d_top[S::KS][2];
+            int t_all = 0;
+            if (TYPE != KV_BF16) {
 #pragma unroll
-            for (int j = 0; j < S::KS; ++j)
+                for (int j = 0; j < S::KS; ++j)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int i = 0; i < 2; ++i) {
+                        d_top[j][i] = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) { on[j][n][i] = true; s[j][n][i] *= factor[n][i & 1]; }
-        }
-        bool grew = false;
-        float m_new[NT][2];
-        int top_new[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float v = m[n][i];
-                int t = top[n][i];
-#pragma unroll
-                for (int j = 0; j < S::KS; ++j) {
-                    v = fmaxf(v, fmaxf(s[j][n][i], s[j][n][i + 2]));
-                    if (TYPE == KV_Q8) {    // NaN scales say nothing here, they make the weight NaN
-                        const float d0 = fabsf(vr[j].d[0][0]), d1 = fabsf(vr[j].d[1][0]);
-                        if (on[j][n][i] && d0 <= 3.4e38f) t = max(t, __float_as_int(d0) & 0x7f800000);
-                        if (on[j][n][i + 2] && d1 <= 3.4e38f) t = max(t, __float_as_int(d1) & 0x7f800000);
+                        for (int g = 0; g < A::G; ++g) d_top[j][i] = fmaxf(d_top[j][i], vr[j].d[i][g]);
                     }
-                }
+                if (!MASKED) {
+                    float d = 0.0f;
 #pragma unroll
-                for (int x = 4; x < 32; x *= 2) {
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
-                    if (TYPE == KV_Q8) t = max(t, __shfl_xor_sync(0xffffffffu, t, x));
+                    for (int j = 0; j < S::KS; ++j) d = fmaxf(d, fmaxf(d_top[j][0], d_top[j][1]));
+                    t_all = __float_as_int(d) & 0x7f800000;
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) t_all = max(t_all, __shfl_xor_sync(0xffffffffu, t_all, x));
                 }
-                m_new[n][i] = v;
-                top_new[n][i] = t;
-                grew |= v > m[n][i] || t > top[n][i];
             }
-        if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float back[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    // nothing seen yet: no sum to scale back
-                    back[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - m_new[n][i]);
-                    l[n][i] *= back[i];
-                    if (TYPE == KV_Q8) {
-                        const int down = (top_new[n][i] - top[n][i]) >> 23;
-                        back[i] *= down > 126 ? 0.0f : __uint_as_float((uint32_t) (127 - down) << 23);
-                    }
-                    m[n][i] = m_new[n][i];
-                    top[n][i] = top_new[n][i];
-                }
-#pragma unroll
-                for (int t = 0; t < S::STEPS; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[t][n][i] *= back[i & 1];
-            }
-        }
-        // ---- outputs: 16 head_dim indexes by 8 NT rows
-#pragma unroll
-        for (int j = 0; j < S::KS; ++j) {
-            float w[NT][4];
+            bool grew = false;
+            float m_new[NT][2];
+            int top_new[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float base = m[n][i & 1] == -INFINITY ? 0.0f : m[n][i & 1];
-                    w[n][i] = fast_exp2(s[j][n][i] - base);
-                    l[n][i & 1] += w[n][i];
-                }
-            uint32_t b[S::PT][NT][2];
-            bool poison = false;
-            if (TYPE == KV_BF16 && masked) {
-                // a value that some rows do not see must not reach them as 0 times infinity
+                for (int i = 0; i < 2; ++i) {
+                    float v = m[n][i];
+                    int t = max(top[n][i], t_all);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int x = 0; x < A::VW; ++x) {
-                        const uint32_t v = vr[j].w[i][x];
-                        poison |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
-                    }
-                poison = __any_sync(0xffffffffu, poison);
-            }
-#pragma unroll
-            for (int t = 0; t < S::STEPS; ++t) {
-                if (t % (S::STEPS / A::G) == 0) {    // the weights times the scales of this group
-                    const int g = t / (S::STEPS / A::G);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float x[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = w[n][i];
-                            if (TYPE == KV_Q8) {    // w * d * 2^(13 - exponent of top) < 2^14
-                                const float norm = __uint_as_float(((254u + 13u) << 23) - (uint32_t) top[n][i & 1]);
-                                x[i] = on[j][n][i] ? w[n][i] * (vr[j].d[i >> 1][0] * norm) : 0.0f;
-                            } else if (TYPE == KV_Q4) {
-                                x[i] = on[j][n][i] ? w[n][i] * vr[j].d[i >> 1][g] : 0.0f;
-                            }
-                        }
-                        uint32_t lo[S::PT], hi[S::PT];
-                        split2<S::BF, S::PT>(x[0], x[1], lo);
-                        split2<S::BF, S::PT>(x[2], x[3], hi);
-#pragma unroll
-                        for (int u = 0; u < S::PT; ++u) {
-                            b[u][n][0] = transpose8x8(lo[u]);
-                            b[u][n][1] = transpose8x8(hi[u]);
+                    for (int j = 0; j < S::KS; ++j) {
+                        v = fmaxf(v, fmaxf(s[j][n][i], s[j][n][i + 2]));
+                        if (TYPE != KV_BF16 && MASKED) {
+                            if (on[j][n][i]) t = max(t, __float_as_int(d_top[j][0]) & 0x7f800000);
+                            if (on[j][n][i + 2]) t = max(t, __float_as_int(d_top[j][1]) & 0x7f800000);
                         }
                     }
-                }
-                uint32_t a[4];
-                value_operand<TYPE, D>(a, vr[j], t);
-                if (TYPE == KV_BF16 && poison) {
-                    // 1 where the value is not finite: its product with the rows that see the key says whose output it spoils
-                    uint32_t bad[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool x = (a[i] & 0x7f80u) == 0x7f80u, y = (a[i] & 0x7f800000u) == 0x7f800000u;
-                        bad[i] = (x ? 0x3f80u : 0u) | (y ? 0x3f800000u : 0u);
-                        a[i] &= (x ? 0u : 0xffffu) | (y ? 0u : 0xffff0000u);
+                    for (int x = 4; x < 32; x *= 2) {
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+                        if (TYPE != KV_BF16 && MASKED) t = max(t, __shfl_xor_sync(0xffffffffu, t, x));
                     }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float spoilt[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-                        const uint32_t see0 = transpose8x8((on[j][n][0] ? 0x3f80u : 0u) | (on[j][n][1] ? 0x3f800000u : 0u));
-                        const uint32_t see1 = transpose8x8((on[j][n][2] ? 0x3f80u : 0u) | (on[j][n][3] ? 0x3f800000u : 0u));
-                        mma16816<true>(spoilt, bad[0], bad[1], bad[2], bad[3], see0, see1);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (spoilt[i] > 0.0f) o[t][n][i] = __uint_as_float(0x7fffffffu);
-                    }
+                    m_new[n][i] = v;
+                    top_new[n][i] = t;
+                    grew |= v > m[n][i] || t > top[n][i];
                 }
+            if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float part[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                    float back[2];
 #pragma unroll
-                    for (int u = S::PT - 1; u >= 0; --u)
-                        mma16816<S::BF>(S::F32 ? part : o[t][n], a[0], a[1], a[2], a[3], b[u][n][0], b[u][n][1]);
-                    if (S::F32)
+                    for (int i = 0; i < 2; ++i) {
+                        // nothing seen yet: no sum to scale back
+                        back[i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - m_new[n][i]);
+                        l[n][i] *= back[i];
+                        if (TYPE != KV_BF16) {
+                            const int down = (top_new[n][i] - top[n][i]) >> 23;
+                            back[i] *= down > 126 ? 0.0f : __uint_as_float((uint32_t) (127 - down) << 23);
+                        }
+                        m[n][i] = m_new[n][i];
+                        top[n][i] = top_new[n][i];
+                    }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[t][n][i] += part[i];
+                    for (int t = 0; t < S::STEPS; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[t][n][i] *= back[i & 1];
                 }
             }
-        }
+            float base[NT][2], norm[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    base[n][i] = m[n][i] == -INFINITY ? 0.0f : m[n][i];
+                    norm[n][i] = __uint_as_float(((254u + 13u) << 23) - (uint32_t) top[n][i]);    // 2^(13 - exponent of top): weights stay below 2^14
+                }
+            // 16 head_dim indexes by 8 NT rows to an instruction
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j) {
+                float w[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        w[n][i] = fast_exp2(s[j][n][i] - base[n][i & 1]);
+                        l[n][i & 1] += w[n][i];
+                        if (TYPE != KV_BF16) w[n][i] *= norm[n][i & 1];
+                    }
+                uint32_t b[S::PT][NT][2];
+                bool poison = false;
+                if (TYPE == KV_BF16 && MASKED) {
+                    // a value that some rows do not see must not reach them as 0 times infinity
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int x = 0; x < A::VW; ++x) {
+                            const uint32_t v = vr[j].w[i][x];
+                            poison |= (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
+                        }
+                    poison = __any_sync(0xffffffffu, poison);
+                }
+#pragma unroll
+                for (int t = 0; t < S::STEPS; ++t) {
+                    if (t % (S::STEPS / A::G) == 0) {    // the weights times the scales of this group
+                        const int g = t / (S::STEPS / A::G);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float x[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                x[i] = w[n][i];
+                                if (TYPE != KV_BF16) x[i] = on[j][n][i] ? w[n][i] * vr[j].d[i >> 1][g] : 0.0f;
+                            }
+                            uint32_t lo[S::PT], hi[S::PT];
+                            split2<S::BF, S::PT>(x[0], x[1], lo);
+                            split2<S::BF, S::PT>(x[2], x[3], hi);
+#pragma unroll
+                            for (int u = 0; u < S::PT; ++u) {
+                                b[u][n][0] = transpose8x8(lo[u]);
+                                b[u][n][1] = transpose8x8(hi[u]);
+                            }
+                        }
+                    }
+                    uint32_t a[4];
+                    value_operand<TYPE, D>(a, vr[j], t);
+                    if (TYPE == KV_BF16 && MASKED && poison) {
+                        // 1 where the value is not finite: its product with the rows that see the key says whose output it spoils
+                        uint32_t bad[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool x = (a[i] & 0x7f80u) == 0x7f80u, y = (a[i] & 0x7f800000u) == 0x7f800000u;
+                            bad[i] = (x ? 0x3f80u : 0u) | (y ? 0x3f800000u : 0u);
+                            a[i] &= (x ? 0u : 0xffffu) | (y ? 0u : 0xffff0000u);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float spoilt[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                            const uint32_t see0 = transpose8x8((on[j][n][0] ? 0x3f80u : 0u) | (on[j][n][1] ? 0x3f800000u : 0u));
+                            const uint32_t see1 = transpose8x8((on[j][n][2] ? 0x3f80u : 0u) | (on[j][n][3] ? 0x3f800000u : 0u));
+                            mma16816<true>(spoilt, bad[0], bad[1], bad[2], bad[3], see0, see1);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (spoilt[i] > 0.0f) o[t][n][i] = __uint_as_float(0x7fffffffu);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float part[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                        for (int u = S::PT - 1; u >= 0; --u)
+                            mma16816<S::BF>(S::F32 ? part : o[t][n], a[0], a[1], a[2], a[3], b[u][n][0], b[u][n][1]);
+                        if (S::F32)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[t][n][i] += part[i];
+                    }
+                }
+            }
+        };
+        if (masked) weigh(std::true_type{});
+        else weigh(std::false_type{});
         if (next < key_end) {
 #pragma unroll
             for (int j = 0; j < S::KS; ++j) load_values<TYPE, D>(vr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
@@ -673,7 +699,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS) attend_kernel(const __grid_co
         float unit[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            unit[i] = TYPE == KV_Q8 ? __uint_as_float((uint32_t) top[n][i] - (13u << 23)) : 1.0f;
+            unit[i] = TYPE != KV_BF16 ? __uint_as_float((uint32_t) top[n][i] - (13u << 23)) : 1.0f;
 #pragma unroll
         for (int t = 0; t < S::STEPS; ++t) {
             const int d = value_dim<TYPE, D>(t, r);

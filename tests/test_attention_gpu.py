@@ -4,7 +4,12 @@ Tolerance, per output: half a step of the output's type relative to the value (b
 sum_j p_j |v_j|:  2 ds for the scores' errors ds (they act on numerator and sum alike), w for the weights' own rounding (to f16, 2^-11, for bf16
 queries; 2^-21 with the exponential's 2 ulp for fp32 ones) and 2^-24 for each of about L / 64 + 64 additions.  ds = (D / 16 + 8) 2^-23 times the
 largest scale sum |q| |k| of the row: a run of D / 16 instructions that drop at most the accumulator's last bit each, and a few roundings
-of the factors around it.  For bf16 queries the output accumulator, too, drops a last bit in each of its L / 64 steps: 2^-23 there."""
+of the factors around it.  For bf16 queries the output accumulator, too, drops a last bit in each of its L / 64 steps: 2^-23 there.
+
+f16 has a smallest step, too.  A weight times its key's scale is an f16 number below 2^14 (2^15 in the kernel for many rows), rounded by at most
+2^-25; the largest weight of a row times the largest scale comes out at 2^13 or more there (2^6 or more), so a key's error is at most 2^-38
+(2^-31) of the largest |v|, and with a second term for fp32 queries 2^-38 as well: L times that on top.  It shows where an output is
+made of weights that small alone: a value of zero at the key that has nearly all the weight."""
 import math
 
 import numpy as np
@@ -69,6 +74,7 @@ class Batch:
                     own = 2.0 ** -21 if f32 else 2.0 ** -11
                     weight = 2 * ds + own + (seen / 64 + 64) * (2.0 ** -24 if f32 else 2.0 ** -23)
                     tol[t] = weight[:, None] * torch.einsum("hk,khd->hd", p, w.abs()) + (2.0 ** -24 if f32 else 2.0 ** -8) * out[t].abs() + 1e-30
+                    tol[t] += seen * (2.0 ** -38 if f32 else 2.0 ** -31) * w.abs().amax(dim=(0, 2))[:, None]
                 t += 1
         return out, lse, tol
 
