@@ -47,7 +47,9 @@ struct AttnParams {
     float scale_log2;                                // scale * log2(e)
     int own_chunk, own_chunks;                       // keys to a chunk, most chunks of a sequence (0: there are no own keys)
     int prefix_chunk, prefix_chunks;
-    int own_prefix;                                  // positions of the prefix that the own keys' kernel walks in front of them (attention_tc.cuh)
+    int own_prefix, own_front;                       // positions of the prefix that the own keys' kernel walks in front of them, and the key number (a
+                                                     // whole number of tiles in attend_kernel) at which the own ones begin
+    int cluster;                                     // the chunks of a row tile are a cluster of blocks, which joins them itself
     int q_aligned, out_aligned;                      // rows start on 16-byte boundaries
     int row_tiles;                                   // of the launch: tiles of rows per sequence (own) or of the whole batch (prefix)
     int direct;                                      // one chunk in all: the block writes the result itself
@@ -274,11 +276,21 @@ __device__ __forceinline__ int value_dim(int tile, int r) {
     return 64 * (tile / 4) + 8 * r + 2 * (tile & 3);
 }
 
-#ifndef ATTN_KS
-#define ATTN_KS 2
-#define ATTN_MB 3
-#endif
 constexpr int ATTN_WARPS = 4;
+
+constexpr int ATTN_CLUSTER = 16;    // most chunks that a cluster joins
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// what block `rank` of the cluster has at this address of its shared memory
+__device__ __forceinline__ float2 cluster_load(const float2 * at, int rank) {
+    float2 v;
+    asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(at)), "r"(rank) : "memory");
+    return v;
+}
 
 template <int TYPE, int D, typename XT, int NT>
 struct AttnShape {
@@ -287,8 +299,8 @@ struct AttnShape {
     static constexpr int QT = F32 ? (BF ? 3 : 2) : 1;                              // terms of a query
     static constexpr int PT = F32 ? (BF ? 3 : 2) : (BF ? 2 : 1);                   // terms of a weight
     static constexpr int STEPS = D / 16;                                           // k steps of the scores, m tiles of the outputs
-    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? ATTN_KS : 1;    // 16-key tiles to a pass of a warp
-    static constexpr int MIN_BLOCKS = D <= 128 && NT == 1 && !F32 ? ATTN_MB : 1;
+    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? 2 : 1;    // 16-key tiles to a pass of a warp
+    static constexpr int MIN_BLOCKS = D <= 128 && NT == 1 && !(F32 && BF) ? 3 : 1;    // to an SM: 168 registers
     static constexpr int ROWS = 8 * NT;
     static constexpr int Q_WORDS = QT * STEPS * NT * 64;
     static constexpr size_t SMEM_Q = Q_WORDS * 4 + ROWS * 8;                       // operands, then factor and reach of every row
@@ -306,14 +318,16 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     float * s_factor = reinterpret_cast<float *>(smem + S::Q_WORDS);
     int * s_seen = reinterpret_cast<int *>(s_factor + S::ROWS);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
-    // row tiles of one chunk are neighbours, so that they share its keys in L2
+    // row tiles of one chunk are neighbours, so that they share its keys in L2; the chunks of a cluster must be
     int at = blockIdx.x;
+    const int chunk_in_cluster = !PREFIX && p.cluster ? at % p.own_chunks : 0;
+    if (!PREFIX && p.cluster) at /= p.own_chunks;
     const int row_tile = at % p.row_tiles;
     at /= p.row_tiles;
     const int head = at % p.kv.n_head;
     at /= p.kv.n_head;
-    const int chunk = PREFIX ? at : at % p.own_chunks;
-    const int seq = PREFIX ? 0 : at / p.own_chunks;
+    const int chunk = PREFIX ? at : p.cluster ? chunk_in_cluster : at % p.own_chunks;
+    const int seq = PREFIX ? 0 : p.cluster ? at : at / p.own_chunks;
 
     // The prefix's kernel lets the own keys' kernel start beside it.  That one reads nothing that the first writes; its block 0 waits for the
     // first to be done, so that what waits for the second waits for both.
@@ -328,9 +342,10 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     }
     const int row0 = row_tile * S::ROWS, n_rows = min(n_new * p.group - row0, S::ROWS);
     const int key0 = chunk * (PREFIX ? p.prefix_chunk : p.own_chunk);
-    if (n_rows <= 0 || (key0 >= len && !(key0 == 0 && p.direct))) return;
-    // keys that a row sees
-    auto reach = [&](int row) { return PREFIX ? len : max(0, len - n_new + (row0 + row) / p.group + 1); };
+    const int front = PREFIX ? 0 : p.own_front;
+    if (n_rows <= 0 || (key0 >= front + len && !(key0 == 0 && p.direct) && (PREFIX || !p.cluster))) return;
+    // keys that a row sees, those between the prefix's end and the own keys' first tile aside
+    auto reach = [&](int row) { return PREFIX ? len : front + max(0, len - n_new + (row0 + row) / p.group + 1); };
     const int key_end = min(key0 + (PREFIX ? p.prefix_chunk : p.own_chunk), reach(n_rows - 1));
     const int seen_by_all = reach(0);
 
@@ -338,8 +353,9 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     const int shift = p.kv.page_shift, in_page = (1 << shift) - 1, n_pages = (int) (p.kv.n_slots >> shift);
     constexpr int STRIDE = 16 * S::KS * ATTN_WARPS;
     // first cache row of a 16-key tile (a page is a whole number of tiles); a page that the cache does not have is reported, its keys count as unseen
-    auto tile_page = [&](int key) { return key < key_end ? table[key >> shift] : 0; };
-    auto tile_row = [&](int page, int key) { return (((int64_t) page * p.kv.n_head + head) << shift) + (key & in_page); };
+    auto place = [&](int key) { return key < front ? key : key - front; };
+    auto tile_page = [&](int key) { return key < key_end ? (key < front ? p.prefix_pages : table)[place(key) >> shift] : 0; };
+    auto tile_row = [&](int page, int key) { return (((int64_t) page * p.kv.n_head + head) << shift) + (place(key) & in_page); };
     KeyRegs<TYPE, D> kr[S::KS];
     ValueRegs<TYPE, D> vr[S::KS];
     int page[S::KS], next_page[S::KS];
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
                     for (int i = 0; i < 4; ++i)
                         s[j][n][i] = TYPE == KV_BF16 ? s[j][n][i] + part[j][n][i] : fmaf(part[j][n][i], kr[j].d[i >> 1][g], s[j][n][i]);
         }
-        bool masked = key + 16 * S::KS > seen_by_all || key + 16 * S::KS > key_end;
+        bool masked = key + 16 * S::KS > seen_by_all || key + 16 * S::KS > key_end || (key < front && key + 16 * S::KS > p.own_prefix);
 #pragma unroll
         for (int j = 0; j < S::KS; ++j) masked |= !good[j];
         bool was_good[S::KS];
@@ -513,7 +529,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int k = key + 16 * j + r + 8 * (i >> 1);
-                        on[j][n][i] = !MASKED || (was_good[j] && k < key_end && k < seen[n][i & 1]);
+                        on[j][n][i] = !MASKED || (was_good[j] && k < key_end && k < seen[n][i & 1] && (k >= front || PREFIX || k < p.own_prefix));
                         s[j][n][i] = on[j][n][i] ? s[j][n][i] * factor[n][i & 1] : -INFINITY;
                     }
             // the largest scale of each key's values; NaN scales say nothing here, they make the weight NaN
@@ -715,8 +731,11 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     }
     __syncthreads();
     const int chunks = p.prefix_chunks + p.own_chunks, slot = PREFIX ? chunk : p.prefix_chunks + chunk;
-    for (int e = threadIdx.x; e < n_rows * (D / 2); e += 32 * ATTN_WARPS) {
-        const int row = e / (D / 2), d = 2 * (e % (D / 2));
+    constexpr int ITEMS = S::ROWS * (D / 2) / (32 * ATTN_WARPS);    // pairs of outputs to a thread
+    float2 out[ITEMS], out_ml[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+        const int e = threadIdx.x + u * 32 * ATTN_WARPS, row = e / (D / 2), d = 2 * (e % (D / 2));
         float most = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
         for (int w = 0; w < ATTN_WARPS; ++w) most = fmaxf(most, sml[w * S::ROWS + row].x);
@@ -727,9 +746,13 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
             const float2 v = *reinterpret_cast<const float2 *>(so + ((size_t) w * S::ROWS + row) * D + d);
             if (ml.x != -INFINITY || ml.y != 0.0f) { sum += ml.y * f; x += v.x * f; y += v.y * f; }
         }
+        out[u] = make_float2(x, y);
+        out_ml[u] = make_float2(most, sum);
+    }
+    auto write = [&](int row, int d, float x, float y, float most, float sum) {
         const int token = first + (row0 + row) / p.group, h = head * p.group + (row0 + row) % p.group;
         const int64_t line = (int64_t) token * p.n_head + h;
-        if (p.direct) {
+        if (p.direct || (!PREFIX && p.cluster)) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             XT * dst = reinterpret_cast<XT *>(p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head) + d;
             dst[0] = from_float<XT>(x * inv);
@@ -739,7 +762,40 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
             *reinterpret_cast<float2 *>(p.part_o + (line * chunks + slot) * D + d) = make_float2(x, y);
             if (d == 0) p.part_ml[line * chunks + slot] = make_float2(most, sum);
         }
+    };
+    if (PREFIX || !p.cluster) {
+#pragma unroll
+        for (int u = 0; u < ITEMS; ++u) {
+            const int e = threadIdx.x + u * 32 * ATTN_WARPS, row = e / (D / 2);
+            if (row < n_rows) write(row, 2 * (e % (D / 2)), out[u].x, out[u].y, out_ml[u].x, out_ml[u].y);
+        }
+        return;
     }
+    // ---- a cluster's blocks read one another's results from shared memory and write a share of the outputs each: nothing goes through the
+    // workspace, and no second kernel has to be launched
+    __syncthreads();
+    float2 * res_ml = reinterpret_cast<float2 *>(so + S::ROWS * D);
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+        const int e = threadIdx.x + u * 32 * ATTN_WARPS, row = e / (D / 2), d = 2 * (e % (D / 2));
+        *reinterpret_cast<float2 *>(so + row * D + d) = out[u];
+        if (d == 0) res_ml[row] = out_ml[u];
+    }
+    cluster_sync();
+    for (int e = chunk * 32 * ATTN_WARPS + threadIdx.x; e < n_rows * (D / 2); e += p.own_chunks * 32 * ATTN_WARPS) {
+        const int row = e / (D / 2), d = 2 * (e % (D / 2));
+        float most = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < p.own_chunks; ++i) most = fmaxf(most, cluster_load(res_ml + row, i).x);
+#pragma unroll 4
+        for (int i = 0; i < p.own_chunks; ++i) {
+            const float2 ml = cluster_load(res_ml + row, i), v = cluster_load(reinterpret_cast<const float2 *>(so + row * D + d), i);
+            const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - most);
+            if (ml.x != -INFINITY || ml.y != 0.0f) { sum += ml.y * f; x += v.x * f; y += v.y * f; }
+        }
+        write(row, d, x, y, most, sum);
+    }
+    cluster_sync();    // nobody leaves while its results are being read
 }
 
 // Joins the chunks of a (token, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.  WARPS warps to a row: one where there are few chunks,
@@ -768,7 +824,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
     }
     int first, n_new, len;
     if (seq >= p.n_seq || !attn_sequence(p, seq, first, n_new, len, false) || token < first || token >= first + n_new) return;    // a row that belongs to nobody
-    const int reach = p.own_prefix + max(0, len - n_new + (token - first) + 1);
+    const int reach = p.own_front + max(0, len - n_new + (token - first) + 1);
     const int own = (reach + p.own_chunk - 1) / p.own_chunk;
     const int n = p.prefix_chunks + own, chunks = p.prefix_chunks + p.own_chunks;
     const float2 * ml = p.part_ml + line * chunks;

@@ -31,11 +31,25 @@ int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int b
     cfg.blockDim = dim3(32 * ATTN_WARPS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = overlap ? 1 : 0;
+    cfg.numAttrs = 0;
+    if (overlap) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (!PREFIX && p.cluster) {
+        static bool wide[ATTN_MAX_DEVICES] = {};    // clusters of more than eight blocks, once for the (function, device) pair
+        if (ctx->device < 0 || ctx->device >= ATTN_MAX_DEVICES) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "device ordinal %d out of range", ctx->device);
+        if (!wide[ctx->device]) {
+            CUDA_TRY(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            wide[ctx->device] = true;
+        }
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned) p.own_chunks;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
     CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kern, p));
     return check_launch(ctx, "attention");
 }

@@ -130,10 +130,12 @@ int kv_move(b200moe_ctx * c, const b200moe_kv_cache * cache, const b200moe_tenso
 struct AttnPlan {
     int own_nt, own_tiles, own_chunk, own_chunks;    // nt: rows to a tile / 8
     int prefix_nt, prefix_tiles, prefix_chunk, prefix_chunks;
-    int own_prefix;
+    int own_prefix, own_front, cluster;
     size_t part_o, bytes;
 };
 
+// Most keys to a block of a cluster.
+constexpr int CLUSTER_KEYS = 1024;
 // Up to so many chunks a row is joined by one warp.
 constexpr int JOIN_FEW = 16;
 // From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries).
@@ -188,9 +190,25 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     pl.own_nt = own_tc ? TC_TILE : tile_units(own_rows, most);
     auto tiles = [&](int64_t n, int nt) { const int tile = nt == TC_TILE ? attend_tc_rows(c->head_dim) : 8 * nt; return (int) ((n + tile - 1) / tile); };
     pl.own_tiles = tiles(own_rows, pl.own_nt);
-    const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles, own_len = (int64_t) a->max_kv_len + pl.own_prefix;
-    if (own_tc) split_keys_tc(own_len, own_base, ctx->sm_count, pl.own_chunk, pl.own_chunks);
-    else split_keys(own_len, own_base, blocks, pass, pl.own_chunk, pl.own_chunks);
+    const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles;
+    // a prefix that is short beside the own keys, or behind which there is one sequence, is walked as well where that reads little twice
+    if (a->prefix_len && !own_tc && (int64_t) a->prefix_len * (a->n_seq - 1) <= (int64_t) a->n_seq * a->max_kv_len / 4) pl.own_prefix = a->prefix_len;
+    pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
+    const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
+    if (own_tc) {
+        split_keys_tc(own_len, own_base, ctx->sm_count, pl.own_chunk, pl.own_chunks);
+    } else {
+        split_keys(own_len, own_base, blocks, pass, pl.own_chunk, pl.own_chunks);
+        // Few blocks: clusters of chunks that join themselves, while all of them are resident together and a block has not too many keys
+        const int64_t most_blocks = (f32 || c->head_dim == 256 ? 2 : 3) * (int64_t) ctx->sm_count;
+        if (pl.own_chunks > 1 && (pl.own_prefix || !a->prefix_len)) {
+            const int64_t n = std::min<int64_t>({ ATTN_CLUSTER, most_blocks / std::max<int64_t>(own_base, 1), pl.own_chunks });
+            if (n > 1 && (own_len + n - 1) / n <= CLUSTER_KEYS) {
+                split_keys(own_len, 1, n, pass, pl.own_chunk, pl.own_chunks);
+                pl.cluster = pl.own_chunks > 1;
+            }
+        }
+    }
     pl.own_chunks = std::max(pl.own_chunks, 1);
     if (a->prefix_len && !pl.own_prefix) {
         pl.prefix_nt = prefix_tc ? TC_TILE : tile_units(rows, most);
@@ -203,7 +221,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     if ((int64_t) a->n_seq * c->n_head_kv * pl.own_tiles * pl.own_chunks >= limit || (int64_t) c->n_head_kv * pl.prefix_tiles * pl.prefix_chunks >= limit)
         return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
     const size_t chunks = pl.own_chunks + pl.prefix_chunks, lines = (size_t) n_tokens * n_head;
-    if (chunks > 1) {
+    if (chunks > 1 && !pl.cluster) {
         pl.part_o = lines * chunks * c->head_dim * sizeof(float);
         pl.bytes = pl.part_o + lines * chunks * sizeof(float2);
     }
@@ -350,9 +368,9 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     p.q_start = a->q_start; p.kv_len = a->kv_len; p.pages = a->pages; p.prefix_pages = a->prefix_pages;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.own_chunk = pl.own_chunk; p.own_chunks = pl.own_chunks;
-    p.prefix_chunk = pl.prefix_chunk; p.prefix_chunks = pl.prefix_chunks; p.own_prefix = pl.own_prefix;
+    p.prefix_chunk = pl.prefix_chunk; p.prefix_chunks = pl.prefix_chunks; p.own_prefix = pl.own_prefix; p.own_front = pl.own_front; p.cluster = pl.cluster;
     p.q_aligned = rows_aligned(q); p.out_aligned = rows_aligned(out);
-    p.direct = pl.bytes == 0;
+    p.direct = pl.own_chunks + pl.prefix_chunks == 1;
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + pl.part_o);
     p.err = ctx->d_err;
@@ -377,7 +395,7 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     const bool overlap = pl.prefix_chunks > 0 && pl.prefix_nt != TC_TILE && pl.own_nt != TC_TILE;
     p.row_tiles = pl.own_tiles;
     if (int rc = launch(pl.own_nt, false, overlap, pl.own_tiles * cache->n_head_kv * pl.own_chunks * a->n_seq)) return rc;
-    if (p.direct) return B200MOE_OK;
+    if (p.direct || p.cluster) return B200MOE_OK;
     if (cache->head_dim == 64) return launch_join<64>(ctx, p, f32, st);
     if (cache->head_dim == 128) return launch_join<128>(ctx, p, f32, st);
     return launch_join<256>(ctx, p, f32, st);

@@ -122,7 +122,7 @@ int main() {
 
     // ---- attention
     const b200moe_tensor q8 = { mem, { 128, 8, 3, 1 }, { 2, 256, 2048, 0 } };
-    const b200moe_attn at = { 3, 1, 300, 100, 5, 0.1f, nullptr, ints, ints, ints };
+    const b200moe_attn at = { 3, 1, 300, 5000, 5, 0.1f, nullptr, ints, ints, ints };
     auto attend = [&](auto change) {
         b200moe_kv_cache kv = c;
         b200moe_tensor q = q8, o = q8;

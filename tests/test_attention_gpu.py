@@ -133,6 +133,18 @@ def test_shared_prefix(gpu_ctx, kind, D, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_short_prefix_and_few_blocks(gpu_ctx, kind, D, dtype):
+    """Prefixes that are walked with the own keys, in one block and in clusters of two to sixteen that join themselves."""
+    Batch(gpu_ctx, kind, [100, 7], prefix=37, D=D, dtype=dtype, seed=1).check()
+    Batch(gpu_ctx, kind, [700, 20, 333], prefix=16, D=D, dtype=dtype, seed=2).check()
+    Batch(gpu_ctx, kind, [3], prefix=2500, D=D, dtype=dtype, seed=3).check()
+    Batch(gpu_ctx, kind, [2100, 0], prefix=101, new=[3, 2], n_head=6, n_kv=1, D=D, dtype=dtype, seed=4, page=32).check()
+    Batch(gpu_ctx, kind, [300] * 9, n_head=16, n_kv=8, D=D, dtype=dtype, seed=5).check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new,lens,prefix", [
     ([3], [3], 0),                          # a whole prompt
     ([2, 5, 1, 4], [2, 90, 7, 131], 0),
@@ -403,11 +415,11 @@ def test_rope_write_attend_as_a_decoder_layer_does(gpu_ctx):
 
 
 def test_refusals(gpu_ctx):
-    b = Batch(gpu_ctx, "q8", [30, 200], prefix=50)
+    b = Batch(gpu_ctx, "q8", [30, 200], prefix=500)
     with pytest.raises(B200MoeError):
         b.call(max_kv_len=300)
     with pytest.raises(ValueError):
-        b.call(prefix_len=65)
+        b.call(prefix_len=513)
     with pytest.raises(ValueError):
         b.call(prefix_pages=None)
     with pytest.raises(ValueError):
