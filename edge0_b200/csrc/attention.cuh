@@ -318,21 +318,17 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     float * s_factor = reinterpret_cast<float *>(smem + S::Q_WORDS);
     int * s_seen = reinterpret_cast<int *>(s_factor + S::ROWS);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane / 4, c = lane % 4;
-    // row tiles of one chunk are neighbours, so that they share its keys in L2; the chunks of a cluster must be
-    int at = blockIdx.x;
-    const int chunk_in_cluster = !PREFIX && p.cluster ? at % p.own_chunks : 0;
-    if (!PREFIX && p.cluster) at /= p.own_chunks;
-    const int row_tile = at % p.row_tiles;
-    at /= p.row_tiles;
-    const int head = at % p.kv.n_head;
-    at /= p.kv.n_head;
-    const int chunk = PREFIX ? at : p.cluster ? chunk_in_cluster : at % p.own_chunks;
-    const int seq = PREFIX ? 0 : p.cluster ? at : at / p.own_chunks;
+    // grid: x row tiles and chunks, y heads, z sequences; the chunks of a cluster are neighbours, else the row tiles of a chunk, so that they
+    // share its keys in L2
+    const bool chunks_inside = !PREFIX && p.cluster;
+    const int inner = chunks_inside ? p.own_chunks : p.row_tiles, outer = inner == 1 ? blockIdx.x : blockIdx.x / inner, rest = blockIdx.x - outer * inner;
+    const int row_tile = chunks_inside ? outer : rest, chunk = chunks_inside ? rest : outer;
+    const int head = blockIdx.y, seq = PREFIX ? 0 : blockIdx.z;
 
     // The prefix's kernel lets the own keys' kernel start beside it.  That one reads nothing that the first writes; its block 0 waits for the
     // first to be done, so that what waits for the second waits for both.
     if (PREFIX) pdl_launch_dependents();
-    else if (blockIdx.x == 0) pdl_wait();
+    else if (blockIdx.x + blockIdx.y + blockIdx.z == 0) pdl_wait();
     int first = 0, n_new, len;
     if (PREFIX) {
         n_new = min(max(p.q_start ? p.q_start[p.n_seq] : p.n_seq, 0), p.n_tokens);
@@ -784,14 +780,20 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     cluster_sync();
     for (int e = chunk * 32 * ATTN_WARPS + threadIdx.x; e < n_rows * (D / 2); e += p.own_chunks * 32 * ATTN_WARPS) {
         const int row = e / (D / 2), d = 2 * (e % (D / 2));
+        float2 ml[ATTN_CLUSTER], v[ATTN_CLUSTER];    // all loads in flight together
         float most = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < p.own_chunks; ++i) most = fmaxf(most, cluster_load(res_ml + row, i).x);
-#pragma unroll 4
-        for (int i = 0; i < p.own_chunks; ++i) {
-            const float2 ml = cluster_load(res_ml + row, i), v = cluster_load(reinterpret_cast<const float2 *>(so + row * D + d), i);
-            const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - most);
-            if (ml.x != -INFINITY || ml.y != 0.0f) { sum += ml.y * f; x += v.x * f; y += v.y * f; }
+#pragma unroll
+        for (int i = 0; i < ATTN_CLUSTER; ++i) {
+            const int from = min(i, p.own_chunks - 1);
+            ml[i] = cluster_load(res_ml + row, from);
+            v[i] = cluster_load(reinterpret_cast<const float2 *>(so + row * D + d), from);
+        }
+#pragma unroll
+        for (int i = 0; i < ATTN_CLUSTER; ++i) most = fmaxf(most, ml[i].x);
+#pragma unroll
+        for (int i = 0; i < ATTN_CLUSTER; ++i) {
+            const float f = ml[i].x == -INFINITY ? 0.0f : fast_exp2(ml[i].x - most);
+            if (i < p.own_chunks && (ml[i].x != -INFINITY || ml[i].y != 0.0f)) { sum += ml[i].y * f; x += v[i].x * f; y += v[i].y * f; }
         }
         write(row, d, x, y, most, sum);
     }
@@ -893,12 +895,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
 // One launch for the own keys or the prefix; the kernels are in a translation unit for each type of cache.  nt: rows to a tile / 8, 1, 2 or 4
 // (at most attend_tiles()); overlap: the own keys' kernel starts beside the prefix's.
 template <int TYPE>
-int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st);
+int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, dim3 grid, cudaStream_t st);
 
 // The same for bf16 queries and tiles of attend_tc_rows() rows (attention_tc.cuh), a launch of its own in every case.
 __host__ __device__ constexpr int attend_tc_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }
 template <int TYPE>
-int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, int blocks, cudaStream_t st);
+int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, dim3 grid, cudaStream_t st);
 
 // most rows to a tile / 8: what leaves the outputs and the loads in registers
 inline int attend_tiles(int head_dim, bool f32) { return f32 || head_dim == 256 ? 2 : 4; }

@@ -3,7 +3,7 @@
 
 namespace b200moe {
 
-template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
-template int launch_attend_tc<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
+template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, dim3, cudaStream_t);
+template int launch_attend_tc<KV_BF16>(ContextBase *, const AttnParams &, int, bool, dim3, cudaStream_t);
 
 }  // namespace b200moe

@@ -19,7 +19,7 @@ int raise_shared_limit(ContextBase * ctx, Kern kern, size_t smem, bool (&done)[A
 }
 
 template <int TYPE, int D, typename XT, int NT, bool PREFIX>
-int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int blocks, cudaStream_t st) {
+int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, dim3 grid, cudaStream_t st) {
     auto kern = attend_kernel<TYPE, D, XT, NT, PREFIX>;
     constexpr size_t smem = AttnShape<TYPE, D, XT, NT>::SMEM;
     if (smem > 48 * 1024) {
@@ -27,7 +27,7 @@ int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int b
         if (int rc = raise_shared_limit(ctx, kern, smem, done)) return rc;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned) blocks);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(32 * ATTN_WARPS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -55,42 +55,42 @@ int launch_attend_t(ContextBase * ctx, const AttnParams & p, bool overlap, int b
 }
 
 template <int TYPE, int D, typename XT, bool PREFIX>
-int launch_attend_n(ContextBase * ctx, const AttnParams & p, int nt, bool overlap, int blocks, cudaStream_t st) {
-    if (nt == 1) return launch_attend_t<TYPE, D, XT, 1, PREFIX>(ctx, p, overlap, blocks, st);
-    if (nt == 2) return launch_attend_t<TYPE, D, XT, 2, PREFIX>(ctx, p, overlap, blocks, st);
-    if constexpr (D < 256 && sizeof(XT) == 2) return launch_attend_t<TYPE, D, XT, 4, PREFIX>(ctx, p, overlap, blocks, st);
+int launch_attend_n(ContextBase * ctx, const AttnParams & p, int nt, bool overlap, dim3 grid, cudaStream_t st) {
+    if (nt == 1) return launch_attend_t<TYPE, D, XT, 1, PREFIX>(ctx, p, overlap, grid, st);
+    if (nt == 2) return launch_attend_t<TYPE, D, XT, 2, PREFIX>(ctx, p, overlap, grid, st);
+    if constexpr (D < 256 && sizeof(XT) == 2) return launch_attend_t<TYPE, D, XT, 4, PREFIX>(ctx, p, overlap, grid, st);
     return fail(ctx, B200MOE_ERR_UNSUPPORTED, "no kernel for %d rows to a tile", 8 * nt);
 }
 
 template <int TYPE, int D>
-int launch_attend_d(ContextBase * ctx, const AttnParams & p, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st) {
-    if (f32) return prefix ? launch_attend_n<TYPE, D, float, true>(ctx, p, nt, overlap, blocks, st) : launch_attend_n<TYPE, D, float, false>(ctx, p, nt, overlap, blocks, st);
-    return prefix ? launch_attend_n<TYPE, D, __nv_bfloat16, true>(ctx, p, nt, overlap, blocks, st)
-                  : launch_attend_n<TYPE, D, __nv_bfloat16, false>(ctx, p, nt, overlap, blocks, st);
+int launch_attend_d(ContextBase * ctx, const AttnParams & p, bool f32, int nt, bool prefix, bool overlap, dim3 grid, cudaStream_t st) {
+    if (f32) return prefix ? launch_attend_n<TYPE, D, float, true>(ctx, p, nt, overlap, grid, st) : launch_attend_n<TYPE, D, float, false>(ctx, p, nt, overlap, grid, st);
+    return prefix ? launch_attend_n<TYPE, D, __nv_bfloat16, true>(ctx, p, nt, overlap, grid, st)
+                  : launch_attend_n<TYPE, D, __nv_bfloat16, false>(ctx, p, nt, overlap, grid, st);
 }
 
 template <int TYPE>
-int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, int blocks, cudaStream_t st) {
-    if (head_dim == 64) return launch_attend_d<TYPE, 64>(ctx, p, f32, nt, prefix, overlap, blocks, st);
-    if (head_dim == 128) return launch_attend_d<TYPE, 128>(ctx, p, f32, nt, prefix, overlap, blocks, st);
-    return launch_attend_d<TYPE, 256>(ctx, p, f32, nt, prefix, overlap, blocks, st);
+int launch_attend(ContextBase * ctx, const AttnParams & p, int head_dim, bool f32, int nt, bool prefix, bool overlap, dim3 grid, cudaStream_t st) {
+    if (head_dim == 64) return launch_attend_d<TYPE, 64>(ctx, p, f32, nt, prefix, overlap, grid, st);
+    if (head_dim == 128) return launch_attend_d<TYPE, 128>(ctx, p, f32, nt, prefix, overlap, grid, st);
+    return launch_attend_d<TYPE, 256>(ctx, p, f32, nt, prefix, overlap, grid, st);
 }
 
 template <int TYPE, int D, bool PREFIX>
-int launch_attend_tc_t(ContextBase * ctx, const AttnParams & p, int blocks, cudaStream_t st) {
+int launch_attend_tc_t(ContextBase * ctx, const AttnParams & p, dim3 grid, cudaStream_t st) {
     auto kern = attend_tc_kernel<TYPE, D, PREFIX>;
     constexpr size_t smem = TcShape<TYPE, D>::SMEM;
     static bool done[ATTN_MAX_DEVICES] = {};
     if (int rc = raise_shared_limit(ctx, kern, smem, done)) return rc;
-    kern<<<(unsigned) blocks, TcShape<TYPE, D>::THREADS, smem, st>>>(p);
+    kern<<<grid, TcShape<TYPE, D>::THREADS, smem, st>>>(p);
     return check_launch(ctx, "attention, tiles of many rows");
 }
 
 template <int TYPE>
-int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, int blocks, cudaStream_t st) {
-    if (head_dim == 64) return prefix ? launch_attend_tc_t<TYPE, 64, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 64, false>(ctx, p, blocks, st);
-    if (head_dim == 128) return prefix ? launch_attend_tc_t<TYPE, 128, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 128, false>(ctx, p, blocks, st);
-    return prefix ? launch_attend_tc_t<TYPE, 256, true>(ctx, p, blocks, st) : launch_attend_tc_t<TYPE, 256, false>(ctx, p, blocks, st);
+int launch_attend_tc(ContextBase * ctx, const AttnParams & p, int head_dim, bool prefix, dim3 grid, cudaStream_t st) {
+    if (head_dim == 64) return prefix ? launch_attend_tc_t<TYPE, 64, true>(ctx, p, grid, st) : launch_attend_tc_t<TYPE, 64, false>(ctx, p, grid, st);
+    if (head_dim == 128) return prefix ? launch_attend_tc_t<TYPE, 128, true>(ctx, p, grid, st) : launch_attend_tc_t<TYPE, 128, false>(ctx, p, grid, st);
+    return prefix ? launch_attend_tc_t<TYPE, 256, true>(ctx, p, grid, st) : launch_attend_tc_t<TYPE, 256, false>(ctx, p, grid, st);
 }
 
 }  // namespace b200moe

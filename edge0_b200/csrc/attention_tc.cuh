@@ -302,13 +302,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
     __shared__ volatile int s_abort;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int at = blockIdx.x;
-    const int row_tile = at % p.row_tiles;
-    at /= p.row_tiles;
-    const int head = at % p.kv.n_head;
-    at /= p.kv.n_head;
-    const int chunk = PREFIX ? at : at % p.own_chunks;
-    const int seq = PREFIX ? 0 : at / p.own_chunks;
+    const int chunk = blockIdx.x / p.row_tiles, row_tile = blockIdx.x - chunk * p.row_tiles, head = blockIdx.y, seq = PREFIX ? 0 : blockIdx.z;
     int first = 0, n_new, len;
     const int front = PREFIX ? p.prefix_len : p.own_prefix;    // keys that every row sees, in the prefix's pages
     if (PREFIX) {

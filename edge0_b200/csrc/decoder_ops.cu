@@ -134,6 +134,7 @@ struct AttnPlan {
     size_t part_o, bytes;
 };
 
+constexpr int64_t WALK_BYTES = 8 << 20;
 // Most keys to a block of a cluster.
 constexpr int CLUSTER_KEYS = 1024;
 // Up to so many chunks a row is joined by one warp.
@@ -172,6 +173,7 @@ int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn
     if (n_head % c->n_head_kv) return fail(ctx, B200MOE_ERR_INVALID_ARG, "n_head must be a multiple of n_head_kv");
     if (!std::isfinite(a->scale)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "scale must be finite");
     if ((int64_t) a->pages_stride * c->page_size < a->max_kv_len) return fail(ctx, B200MOE_ERR_INVALID_ARG, "max_kv_len needs more pages than a sequence's table has");
+    if (a->n_seq > 65535 || c->n_head_kv > 65535) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "at most 65535 sequences and as many key/value heads");
     if (a->max_kv_len > INT32_MAX / 4 || a->prefix_len > INT32_MAX / 4) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "at most 2^29 positions");
     if (n_tokens * n_head >= ((int64_t) 1 << 31) || (int64_t) a->max_new * n_head >= ((int64_t) 1 << 31)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
     return B200MOE_OK;
@@ -191,8 +193,10 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     auto tiles = [&](int64_t n, int nt) { const int tile = nt == TC_TILE ? attend_tc_rows(c->head_dim) : 8 * nt; return (int) ((n + tile - 1) / tile); };
     pl.own_tiles = tiles(own_rows, pl.own_nt);
     const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles;
-    // a prefix that is short beside the own keys, or behind which there is one sequence, is walked as well where that reads little twice
-    if (a->prefix_len && !own_tc && (int64_t) a->prefix_len * (a->n_seq - 1) <= (int64_t) a->n_seq * a->max_kv_len / 4) pl.own_prefix = a->prefix_len;
+    // A prefix is walked by every sequence, too, where that reads little twice: the launches and the join that it saves take as long as about 8 MB of
+    // the cache (56 heads, two sequences of 23 keys behind 31: 13.8 us with a launch of its own, 5.8 walked).
+    const int64_t again = (int64_t) a->prefix_len * (a->n_seq - 1) * c->n_head_kv * 2 * row_bytes(c->type, c->head_dim);
+    if (a->prefix_len && !own_tc && (again <= WALK_BYTES || (int64_t) a->prefix_len * (a->n_seq - 1) <= (int64_t) a->n_seq * a->max_kv_len / 4)) pl.own_prefix = a->prefix_len;
     pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
     const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
     if (own_tc) {
@@ -217,8 +221,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
         if (prefix_tc) split_keys_tc(a->prefix_len, base, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
         else split_keys(a->prefix_len, base, one_wave, pass, pl.prefix_chunk, pl.prefix_chunks);
     }
-    const int64_t limit = (int64_t) 1 << 31;
-    if ((int64_t) a->n_seq * c->n_head_kv * pl.own_tiles * pl.own_chunks >= limit || (int64_t) c->n_head_kv * pl.prefix_tiles * pl.prefix_chunks >= limit)
+    if ((int64_t) pl.own_tiles * pl.own_chunks > INT32_MAX || (int64_t) pl.prefix_tiles * pl.prefix_chunks > INT32_MAX)
         return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
     const size_t chunks = pl.own_chunks + pl.prefix_chunks, lines = (size_t) n_tokens * n_head;
     if (chunks > 1 && !pl.cluster) {
@@ -251,12 +254,12 @@ int launch_join(ContextBase * ctx, const AttnParams & p, bool f32, cudaStream_t 
 }  // namespace
 
 namespace b200moe {
-extern template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
-extern template int launch_attend_tc<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
-extern template int launch_attend<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
-extern template int launch_attend_tc<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
-extern template int launch_attend<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, int, cudaStream_t);
-extern template int launch_attend_tc<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, cudaStream_t);
+extern template int launch_attend<KV_BF16>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, dim3, cudaStream_t);
+extern template int launch_attend_tc<KV_BF16>(ContextBase *, const AttnParams &, int, bool, dim3, cudaStream_t);
+extern template int launch_attend<KV_Q8>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, dim3, cudaStream_t);
+extern template int launch_attend_tc<KV_Q8>(ContextBase *, const AttnParams &, int, bool, dim3, cudaStream_t);
+extern template int launch_attend<KV_Q4>(ContextBase *, const AttnParams &, int, bool, int, bool, bool, dim3, cudaStream_t);
+extern template int launch_attend_tc<KV_Q4>(ContextBase *, const AttnParams &, int, bool, dim3, cudaStream_t);
 }  // namespace b200moe
 
 extern "C" {
@@ -376,25 +379,25 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     p.err = ctx->d_err;
     CUDA_TRY(ctx, cudaSetDevice(ctx->device));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    auto launch = [&](int nt, bool prefix, bool overlap, int blocks) {
+    auto launch = [&](int nt, bool prefix, bool overlap, dim3 grid) {
         const int d = cache->head_dim;
         if (nt == TC_TILE) {
-            if (cache->type == KV_BF16) return launch_attend_tc<KV_BF16>(ctx, p, d, prefix, blocks, st);
-            if (cache->type == KV_Q8) return launch_attend_tc<KV_Q8>(ctx, p, d, prefix, blocks, st);
-            return launch_attend_tc<KV_Q4>(ctx, p, d, prefix, blocks, st);
+            if (cache->type == KV_BF16) return launch_attend_tc<KV_BF16>(ctx, p, d, prefix, grid, st);
+            if (cache->type == KV_Q8) return launch_attend_tc<KV_Q8>(ctx, p, d, prefix, grid, st);
+            return launch_attend_tc<KV_Q4>(ctx, p, d, prefix, grid, st);
         }
-        if (cache->type == KV_BF16) return launch_attend<KV_BF16>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
-        if (cache->type == KV_Q8) return launch_attend<KV_Q8>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
-        return launch_attend<KV_Q4>(ctx, p, d, f32, nt, prefix, overlap, blocks, st);
+        if (cache->type == KV_BF16) return launch_attend<KV_BF16>(ctx, p, d, f32, nt, prefix, overlap, grid, st);
+        if (cache->type == KV_Q8) return launch_attend<KV_Q8>(ctx, p, d, f32, nt, prefix, overlap, grid, st);
+        return launch_attend<KV_Q4>(ctx, p, d, f32, nt, prefix, overlap, grid, st);
     };
     if (pl.prefix_chunks) {
         p.row_tiles = pl.prefix_tiles;
-        if (int rc = launch(pl.prefix_nt, true, false, pl.prefix_tiles * cache->n_head_kv * pl.prefix_chunks)) return rc;
+        if (int rc = launch(pl.prefix_nt, true, false, dim3(pl.prefix_tiles * pl.prefix_chunks, cache->n_head_kv, 1))) return rc;
     }
     // nothing becomes resident beside a kernel that holds tensor memory
     const bool overlap = pl.prefix_chunks > 0 && pl.prefix_nt != TC_TILE && pl.own_nt != TC_TILE;
     p.row_tiles = pl.own_tiles;
-    if (int rc = launch(pl.own_nt, false, overlap, pl.own_tiles * cache->n_head_kv * pl.own_chunks * a->n_seq)) return rc;
+    if (int rc = launch(pl.own_nt, false, overlap, dim3(pl.own_tiles * pl.own_chunks, cache->n_head_kv, a->n_seq))) return rc;
     if (p.direct || p.cluster) return B200MOE_OK;
     if (cache->head_dim == 64) return launch_join<64>(ctx, p, f32, st);
     if (cache->head_dim == 128) return launch_join<128>(ctx, p, f32, st);

@@ -122,7 +122,7 @@ int main() {
 
     // ---- attention
     const b200moe_tensor q8 = { mem, { 128, 8, 3, 1 }, { 2, 256, 2048, 0 } };
-    const b200moe_attn at = { 3, 1, 300, 5000, 5, 0.1f, nullptr, ints, ints, ints };
+    const b200moe_attn at = { 3, 1, 300, 50000, 5, 0.1f, nullptr, ints, ints, ints };
     auto attend = [&](auto change) {
         b200moe_kv_cache kv = c;
         b200moe_tensor q = q8, o = q8;
@@ -164,6 +164,7 @@ int main() {
     ATTEND(UNSUP, a.prefix_len = INT32_MAX);
     ATTEND(UNSUP, q.ne[2] = o.ne[2] = (int64_t) 1 << 29, a.q_start = ints);
     ATTEND(UNSUP, kv.page_size = 20);
+    ATTEND(UNSUP, a.n_seq = 65536, a.q_start = ints);
     ATTEND(ARG, kv.k = nullptr);
     size_t need = 0;
     expect("workspace", b200moe_attention_workspace(ctx, &c, &at, 8, 3, &need), OK);

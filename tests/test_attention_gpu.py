@@ -126,8 +126,9 @@ def test_pages_that_end_inside_a_tile(gpu_ctx, kind, page):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_shared_prefix(gpu_ctx, kind, D, dtype):
-    Batch(gpu_ctx, kind, [5, 90, 1, 44], prefix=1000, D=D, dtype=dtype, seed=1).check()
-    Batch(gpu_ctx, kind, [5] * 33, prefix=333, D=D, dtype=dtype, seed=2).check()
+    Batch(gpu_ctx, kind, [5, 90, 1, 44], prefix=1000, n_head=160, n_kv=40, D=D, dtype=dtype, seed=1).check()
+    Batch(gpu_ctx, kind, [5] * 33, prefix=333, n_head=20, n_kv=10, D=D, dtype=dtype, seed=2).check()
+    Batch(gpu_ctx, kind, [5] * 33, prefix=1777, D=D, dtype=dtype, seed=2).check()
     Batch(gpu_ctx, kind, [20], prefix=1, D=D, dtype=dtype, seed=3).check()
 
 
@@ -415,7 +416,7 @@ def test_rope_write_attend_as_a_decoder_layer_does(gpu_ctx):
 
 
 def test_refusals(gpu_ctx):
-    b = Batch(gpu_ctx, "q8", [30, 200], prefix=500)
+    b = Batch(gpu_ctx, "q8", [30, 200], prefix=500, n_head=66, n_kv=66)
     with pytest.raises(B200MoeError):
         b.call(max_kv_len=300)
     with pytest.raises(ValueError):
@@ -433,7 +434,7 @@ def test_refusals(gpu_ctx):
     with pytest.raises(TypeError):
         b.call(q=b.q.half())
     with pytest.raises(B200MoeError):
-        b.call(q=b.q[:, :7])
+        b.call(q=b.q[:, :65])
     with pytest.raises(B200MoeError):
         b.call(q=b.q[..., :64].contiguous())
     with pytest.raises(B200MoeError):
