@@ -299,7 +299,7 @@ struct AttnShape {
     static constexpr int QT = F32 ? (BF ? 3 : 2) : 1;                              // terms of a query
     static constexpr int PT = F32 ? (BF ? 3 : 2) : (BF ? 2 : 1);                   // terms of a weight
     static constexpr int STEPS = D / 16;                                           // k steps of the scores, m tiles of the outputs
-    static constexpr int KS = TYPE != KV_BF16 && D <= 128 && !F32 && NT == 1 ? 2 : 1;    // 16-key tiles to a pass of a warp
+    static constexpr int KS = NT == 1 && !F32 && (D == 64 || (TYPE != KV_BF16 && D == 128)) ? 2 : 1;    // 16-key tiles to a pass of a warp
     static constexpr int MIN_BLOCKS = D <= 128 && NT == 1 && !(F32 && BF) ? 3 : 1;    // to an SM: 168 registers
     static constexpr int ROWS = 8 * NT;
     static constexpr int Q_WORDS = QT * STEPS * NT * 64;

@@ -204,7 +204,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     } else {
         split_keys(own_len, own_base, blocks, pass, pl.own_chunk, pl.own_chunks);
         // Few blocks: clusters of chunks that join themselves, while all of them are resident together and a block has not too many keys
-        const int64_t most_blocks = (f32 || c->head_dim == 256 ? 2 : 3) * (int64_t) ctx->sm_count;
+        const int64_t most_blocks = (c->head_dim == 256 || (f32 && c->type == KV_BF16 && c->head_dim == 128) ? 2 : 3) * (int64_t) ctx->sm_count;
         if (pl.own_chunks > 1 && (pl.own_prefix || !a->prefix_len)) {
             const int64_t n = std::min<int64_t>({ ATTN_CLUSTER, most_blocks / std::max<int64_t>(own_base, 1), pl.own_chunks });
             if (n > 1 && (own_len + n - 1) / n <= CLUSTER_KEYS) {
