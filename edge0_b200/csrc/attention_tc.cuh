@@ -192,7 +192,8 @@ __device__ __forceinline__ void tc_load(TcPiece<TYPE, D> & t, const uint8_t * ro
     typedef TcShape<TYPE, D> S;
 #pragma unroll
     for (int n = 0; n < S::NL; ++n) {
-        t.v[n] = make_uint4(0, 0, 0, 0);
+        constexpr uint32_t ZERO = TYPE == KV_Q8 ? 0x80808080u : 0u;    // codes of a row that is not there
+        t.v[n] = make_uint4(ZERO, ZERO, ZERO, ZERO);
         const int64_t row = kv_row(kv, max(slot[n], 0), head);
         if (slot[n] >= 0) t.v[n] = load_stream(reinterpret_cast<const uint4 *>(rows + row * kv_row_bytes<TYPE, D>() + 16 * x));
         if (TYPE == KV_Q8) t.s[n][0] = slot[n] >= 0 ? static_cast<const uint32_t *>(scales)[row] : 0u;
@@ -212,8 +213,8 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
         uint32_t h[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            h[2 * i] = there ? bytes_to_half2(w[i], 0x4140) : 0u;
-            h[2 * i + 1] = there ? bytes_to_half2(w[i], 0x4342) : 0u;
+            h[2 * i] = bytes_to_half2(w[i], 0x4140);
+            h[2 * i + 1] = bytes_to_half2(w[i], 0x4342);
         }
         lo = make_uint4(h[0], h[1], h[2], h[3]);
         hi = make_uint4(h[4], h[5], h[6], h[7]);
@@ -293,6 +294,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
     uint8_t * sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t) 1023);
     uint8_t * sk = sq + GROUPS * S::Q_BYTES, * sv = sk + NS * S::KV_BYTES;
     __shared__ uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS];
+    __shared__ uint64_t turn[2][4];    // [group][warp of the group]: its turn at the exponentials
     __shared__ uint64_t q_full, s_full[2 * GROUPS], p_full[2 * GROUPS], pv_done[2 * GROUPS];    // [group][parity of the tile]
     __shared__ __align__(16) float k_scale[NS][KT], v_scale[NS][KT];
     __shared__ float s_factor[GROUPS * TC_GROUP_ROWS];
@@ -334,6 +336,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             mbar_init(&p_full[i], TC_GROUP_ROWS);
             mbar_init(&pv_done[i], 1);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(&turn[i / 4][i % 4], 1);
         mbar_init(&q_full, 32 * SW);
         mbar_fence_init();
         s_abort = 0;
@@ -353,32 +356,43 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
         constexpr int TPR = D / 8, PASS = 32 * SW / TPR, BATCH = GROUPS * TC_GROUP_ROWS / PASS < 16 ? GROUPS * TC_GROUP_ROWS / PASS : 16;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
         const int x = tid % TPR;
+        // row r of the block is head_at of token_at, PASS rows on the same with these steps
+        int token_at = first + (row0 + tid / TPR) / p.group, head_at = (row0 + tid / TPR) % p.group;
+        const int token_step = PASS / p.group, head_step = PASS % p.group;
 #pragma unroll 1
         for (int r0 = 0; r0 < GROUPS * TC_GROUP_ROWS; r0 += PASS * BATCH) {
             uint4 raw[BATCH];
+            const char * src[BATCH];
 #pragma unroll
             for (int n = 0; n < BATCH; ++n) {
-                const int row = r0 + n * PASS + tid / TPR, at_row = row0 + min(row, n_rows - 1);
-                const int token = first + at_row / p.group, h = head * p.group + at_row % p.group;
-                const char * src = p.q + (int64_t) token * p.q_token + (int64_t) h * p.q_head + 16 * x;
-                if (p.q_aligned) {
-                    raw[n] = *reinterpret_cast<const uint4 *>(src);
-                } else {
-                    const uint16_t * e = reinterpret_cast<const uint16_t *>(src);
+                const bool there = r0 + n * PASS + tid / TPR < n_rows;    // else the first row, whose values are not used
+                src[n] = p.q + (int64_t) (there ? token_at : first + row0 / p.group) * p.q_token + (int64_t) (head * p.group + (there ? head_at : 0)) * p.q_head + 16 * x;
+                token_at += token_step;
+                head_at += head_step;
+                if (head_at >= p.group) { head_at -= p.group; ++token_at; }
+            }
+            if (p.q_aligned) {    // no branch between the loads: all of them in flight
+#pragma unroll
+                for (int n = 0; n < BATCH; ++n) raw[n] = *reinterpret_cast<const uint4 *>(src[n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < BATCH; ++n) {
+                    const uint16_t * e = reinterpret_cast<const uint16_t *>(src[n]);
                     raw[n] = make_uint4(e[0] | (uint32_t) e[1] << 16, e[2] | (uint32_t) e[3] << 16, e[4] | (uint32_t) e[5] << 16, e[6] | (uint32_t) e[7] << 16);
                 }
-                if (row >= n_rows) raw[n] = make_uint4(0, 0, 0, 0);
             }
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n)
+                if (r0 + n * PASS + tid / TPR >= n_rows) raw[n] = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int n = 0; n < BATCH; ++n) {
                 const int row = r0 + n * PASS + tid / TPR;
                 const uint32_t w[4] = { raw[n].x, raw[n].y, raw[n].z, raw[n].w };
-                float most = 0.0f;    // NaN says nothing about the size
+                // sizes as bf16 bits, two to a word: they have the numbers' order
+                uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-#pragma unroll
-                for (int o = TPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float up = row_up(__float_as_uint(most));
+                for (int o = TPR / 2; o > 0; o >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float up = row_up(max(most << 16, most & 0xffff0000u));
                 uint32_t h2[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -478,7 +492,12 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                         }
                     }
                 }
-                // the weights, over the scores
+                // The weights, over the scores.  The two groups' warps of a scheduler take turns here: together they would wait for the exponentials at
+                // the same time and for everything else at the same time, too (a tile 3,000 cycles, MEASURED in turns).
+                if (n_groups == 2) {
+                    ok = __all_sync(0xffffffffu, wait_suspended(&turn[group][warp & 3], group == 0 ? (i & 1) ^ 1u : i & 1, &s_abort, p.err));
+                    if (!ok) break;
+                }
                 const float base = ref == -INFINITY ? 0.0f : -ref;
                 const uint64_t base2 = pack2(base, base), factor2 = pack2(factor, factor);
                 if (!masked) {
@@ -508,6 +527,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                         s[0][c / 2] = half2_bits(__floats2half2_rn(v[0], v[1]));
                     }
                 }
+                if (n_groups == 2 && lane == 0) mbar_arrive(&turn[group ^ 1][warp & 3]);
                 tmem_store32(t_s, s[0]);
                 tmem_wait_st();
                 tc_fence_before();
@@ -531,11 +551,15 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                 const int chunks = p.prefix_chunks + p.own_chunks, slot = PREFIX ? chunk : p.prefix_chunks + chunk;
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const bool there = row < n_rows;
-                // 32 by 32 values at a time through the group's query tile, which nothing reads any more, so that a row's values leave together
-                float * stage = reinterpret_cast<float *>(sq + group * S::Q_BYTES + (warp & 3) * 4096);
-                // where the thread's row goes; the warp's threads tell one another
-                const int64_t to = p.direct ? (int64_t) token * p.out_token + (int64_t) h * p.out_head : (line * chunks + slot) * (int64_t) (D * 4);
-                const int in_warp = min(32, n_rows - warp * 32);    // rows of this warp
+                // 32 by 32 values at a time through the group's query tile, which nothing reads any more, so that a row's values leave together:
+                // 16-byte pieces, piece k of a row at k ^ (row & 7), eight lanes to a row of what is stored
+                uint4 * stage = reinterpret_cast<uint4 *>(sq + group * S::Q_BYTES + (warp & 3) * 4096);
+                const int64_t mine = p.direct ? (int64_t) token * p.out_token + (int64_t) h * p.out_head : (line * chunks + slot) * (int64_t) (D * 4);
+                char * const base = p.direct ? p.out : reinterpret_cast<char *>(p.part_o);
+                const int in_warp = n_rows - warp * 32, piece = lane & 7;    // rows of this warp
+                int64_t to[8];    // where rows 4i + lane / 8 go
+#pragma unroll
+                for (int i = 0; i < 8; ++i) to[i] = __shfl_sync(0xffffffffu, mine, 4 * i + (lane >> 3));
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
@@ -546,31 +570,30 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] = 0u;
                     }
+                    if (p.direct) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
+                    }
                     __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        stage[lane * 32 + (j ^ lane)] = !p.direct ? __uint_as_float(o[j]) : sum == 0.0f ? 0.0f : __uint_as_float(o[j]) * inv;
+                    for (int k = 0; k < 8; ++k) stage[lane * 8 + (k ^ (lane & 7))] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
                     __syncwarp();
-                    if (!p.direct) {
-#pragma unroll 8
-                        for (int r = 0; r < 32; ++r) {
-                            const int64_t at_row = __shfl_sync(0xffffffffu, to, r);
-                            if (r < in_warp) *reinterpret_cast<float *>(reinterpret_cast<char *>(p.part_o) + at_row + (c + lane) * 4) = stage[r * 32 + (lane ^ r)];
-                        }
-                    } else {
-#pragma unroll 8
-                        for (int r2 = 0; r2 < 32; r2 += 2) {
-                            const int r = r2 + (lane >> 4), d = 2 * (lane & 15);
-                            const int64_t at_row = __shfl_sync(0xffffffffu, to, r);
-                            const __nv_bfloat162 v = __floats2bfloat162_rn(stage[r * 32 + (d ^ r)], stage[r * 32 + ((d + 1) ^ r)]);
-                            char * dst = p.out + at_row + (c + d) * 2;
-                            if (r < in_warp) {
-                                if (p.out_aligned) {
-                                    *reinterpret_cast<__nv_bfloat162 *>(dst) = v;
-                                } else {
-                                    reinterpret_cast<__nv_bfloat16 *>(dst)[0] = v.x;
-                                    reinterpret_cast<__nv_bfloat16 *>(dst)[1] = v.y;
-                                }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + (lane >> 3);
+                        const uint4 v = stage[r * 8 + (piece ^ (r & 7))];
+                        if (r >= in_warp) continue;
+                        if (!p.direct) {
+                            *reinterpret_cast<uint4 *>(base + to[i] + (c + 4 * piece) * 4) = v;
+                        } else {
+                            const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(v.x), __uint_as_float(v.y));
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(v.z), __uint_as_float(v.w));
+                            char * dst = base + to[i] + (c + 4 * piece) * 2;
+                            if (p.out_aligned) {
+                                *reinterpret_cast<uint2 *>(dst) = make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
+                            } else {
+                                __nv_bfloat16 * e = reinterpret_cast<__nv_bfloat16 *>(dst);
+                                e[0] = x.x; e[1] = x.y; e[2] = y.x; e[3] = y.y;
                             }
                         }
                     }

@@ -138,7 +138,7 @@ constexpr int64_t WALK_BYTES = 8 << 20;
 // Most keys to a block of a cluster.
 constexpr int CLUSTER_KEYS = 1024;
 // Up to so many chunks a row is joined by one warp.
-constexpr int JOIN_FEW = 16;
+constexpr int JOIN_FEW = 32;
 // From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries).
 constexpr int ATTN_TC_ROWS = 64;
 constexpr int TC_TILE = 0;     // nt of those kernels, whose tile goes by the head_dim
