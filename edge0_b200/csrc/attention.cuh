@@ -8,11 +8,12 @@
 // maximum and sum of its own, and join at the end; chunks (and the prefix) are joined by attend_join_kernel through the workspace.
 //
 // Products run on mma.m16n8k16 with the keys on the M side: S^T = K Q^T has 16 keys by 8 rows to an instruction, so the 8 query heads of
-// a key/value head fill it, and O^T = V^T P^T takes its second operand from S^T by one 8x8 transpose between lanes.  A lane's share of K and
-// of V^T is loaded from global memory straight into registers in 4 to 16-byte pieces that together cover whole sectors of the cache's rows: no
-// shared memory on the way, no barrier in the loop, the loads of the next keys fly while this step's values are multiplied.
+// a key/value head fill it, and O^T = V^T P^T takes its second operand from S^T by one 8x8 transpose between lanes.
 //   Keys: lane (r = lane / 4, c = lane % 4) holds keys r and r + 8 of a tile; any order of head_dim serves as the k index as long as Q has
 //   the same, so a lane's pieces are contiguous.  Values: it holds keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them by byte permutes.
+// Every warp has a ring of two or three passes of its own in shared memory, filled by asynchronous 16-byte copies that run while the passes
+// before are worked on (two thirds of what 227 KB hold is in flight; a register's worth ahead, as before, was 48 KB an SM and 2.9 TB/s); no barrier in
+// the loop.  Pieces of a row lie at piece ^ swizzle(row), so that both kinds of reads meet no bank conflicts on rows of 128 bytes and more.
 //
 // Precision.  The codes are whole numbers and go into the product exactly; the scales stay outside in fp32: a key's multiplies the score,
 // a value's the weight p.  Q8 and Q4: codes as f16 (a byte or nibble under the exponent of 1024), queries as f16 with a power of two to a row that
@@ -160,42 +161,79 @@ struct KeyRegs {
     float d[2][A::G];    // scales (Q8 as they are; Q4 widened when used)
 };
 
+// 16-byte piece of a row where another lies without swizzle: neighbouring rows differ in bit 2, the even ones in bits 1 and 2 (lanes read the keys'
+// rows two at a time, the values' even or odd rows four at a time)
+__device__ __forceinline__ int tile_swizzle(int row, int pieces) { return ((row & 6) ^ (row & 1 ? 5 : 0)) & (pieces < 8 ? pieces - 1 : 7); }
+
+__device__ __forceinline__ void copy_async16(void * to, const void * from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void * to, const void * from) {
+    if constexpr (BYTES == 16) copy_async16(to, from);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES) : "memory");
+}
+
+// a 16-key tile in shared memory: keys' rows, values' rows, the keys' scales, the values' scales
 template <int TYPE, int D>
-__device__ __forceinline__ void load_scales(float (&d)[AttnTile<TYPE, D>::G], const void * scales, int64_t row) {
-    if (TYPE == KV_Q8) {
-        d[0] = static_cast<const float *>(scales)[row];
-    } else if (TYPE == KV_Q4) {
+struct TileBytes {
+    static constexpr int RB = kv_row_bytes<TYPE, D>(), PIECES = RB / 16;
+    static constexpr int SB = TYPE == KV_Q8 ? 4 : TYPE == KV_Q4 ? D / 16 : 0;    // scales of a row
+    static constexpr int V = 16 * RB, KS = 32 * RB, VS = KS + 16 * SB, ALL = KS + 32 * SB;
+};
+
+// the warp begins to copy the tile of cache rows row0 .. row0 + 15
+template <int TYPE, int D>
+__device__ __forceinline__ void fill_tile(uint8_t * tile, const KvView & kv, int64_t row0, int lane) {
+    typedef TileBytes<TYPE, D> B;
+#pragma unroll
+    for (int n = 0; n < B::RB; n += 32) {    // B::RB pieces in all
+        const int q = n + lane, row = q / B::PIECES, piece = q % B::PIECES, to = row * B::RB + ((piece ^ tile_swizzle(row, B::PIECES)) << 4);
+        copy_async16(tile + to, kv.k + row0 * B::RB + q * 16);
+        copy_async16(tile + B::V + to, kv.v + row0 * B::RB + q * 16);
+    }
+    if constexpr (B::SB > 0)
+        copy_async<B::SB>(tile + B::KS + lane * B::SB,
+                          static_cast<const uint8_t *>(lane < 16 ? kv.k_scale : kv.v_scale) + (row0 + (lane & 15)) * B::SB);
+}
+
+template <int TYPE, int D>
+__device__ __forceinline__ void load_scales(float (&d)[AttnTile<TYPE, D>::G], const uint8_t * scales, int row) {
+    typedef TileBytes<TYPE, D> B;
+    if constexpr (TYPE == KV_Q8) {
+        d[0] = *reinterpret_cast<const float *>(scales + row * B::SB);
+    } else if constexpr (TYPE == KV_Q4) {
         constexpr int G = AttnTile<TYPE, D>::G;
-        const uint32_t * p = reinterpret_cast<const uint32_t *>(static_cast<const __nv_bfloat16 *>(scales) + row * G);
+        const Pack<uint32_t, G / 2> w = *reinterpret_cast<const Pack<uint32_t, G / 2> *>(scales + row * B::SB);
 #pragma unroll
         for (int g = 0; g < G; g += 2) {
-            const uint32_t w = p[g / 2];
-            d[g] = __uint_as_float(w << 16);
-            d[(g + 1) % G] = __uint_as_float(w & 0xffff0000u);
+            d[g] = __uint_as_float(w.v[g / 2] << 16);
+            d[g + 1] = __uint_as_float(w.v[g / 2] & 0xffff0000u);
         }
     }
 }
 
 template <int TYPE, int D>
-__device__ __forceinline__ void load_keys(KeyRegs<TYPE, D> & t, const KvView & kv, int64_t row0, int lane) {
+__device__ __forceinline__ void load_keys(KeyRegs<TYPE, D> & t, const uint8_t * tile, int lane) {
     typedef AttnTile<TYPE, D> A;
+    typedef TileBytes<TYPE, D> B;
     const int r = lane / 4, c = lane % 4;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int64_t row = row0 + r + 8 * i;
-        const uint8_t * at = kv.k + row * A::RB;
+        const int row = r + 8 * i, x = tile_swizzle(row, B::PIECES);
+        const uint8_t * at = tile + row * B::RB;
 #pragma unroll
         for (int w = 0; w < A::KW; w += A::KP) {
             // pieces of the four lanes lie side by side
             if constexpr (A::KP == 4) {
-                const uint4 v = load_stream(reinterpret_cast<const uint4 *>(at + 16 * w + 16 * c));
+                const uint4 v = *reinterpret_cast<const uint4 *>(at + (((w + c) ^ x) << 4));
                 t.w[i][w] = v.x; t.w[i][w + 1] = v.y; t.w[i][w + 2] = v.z; t.w[i][w + 3] = v.w;
             } else {
-                const uint2 v = load_stream(reinterpret_cast<const uint2 *>(at + 16 * w + 8 * c));
+                const uint2 v = *reinterpret_cast<const uint2 *>(at + ((c / 2 ^ x) << 4) + 8 * (c % 2));
                 t.w[i][w] = v.x; t.w[i][w + 1] = v.y;
             }
         }
-        load_scales<TYPE, D>(t.d[i], kv.k_scale, row);
+        load_scales<TYPE, D>(t.d[i], tile + B::KS, row);
     }
 }
 
@@ -207,29 +245,31 @@ struct ValueRegs {
 };
 
 template <int TYPE, int D>
-__device__ __forceinline__ void load_values(ValueRegs<TYPE, D> & t, const KvView & kv, int64_t row0, int lane) {
+__device__ __forceinline__ void load_values(ValueRegs<TYPE, D> & t, const uint8_t * tile, int lane) {
     typedef AttnTile<TYPE, D> A;
+    typedef TileBytes<TYPE, D> B;
     const int r = lane / 4, c = lane % 4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t row = row0 + 2 * c + (i & 1) + 8 * (i >> 1);
-        const uint8_t * at = kv.v + row * A::RB;
+        const int row = 2 * c + (i & 1) + 8 * (i >> 1), x = tile_swizzle(row, B::PIECES);
+        const uint8_t * at = tile + B::V + row * B::RB;
 #pragma unroll
         for (int w = 0; w < A::VW; w += A::VP) {
-            const uint8_t * piece = at + 32 * w + 4 * A::VP * r;
+            const int byte = 32 * w + 4 * A::VP * r;
+            const uint8_t * piece = at + ((byte / 16 ^ x) << 4) + byte % 16;
             if constexpr (A::VP == 4) {
-                const uint4 v = load_stream(reinterpret_cast<const uint4 *>(piece));
+                const uint4 v = *reinterpret_cast<const uint4 *>(piece);
                 t.w[i][w] = v.x; t.w[i][w + 1] = v.y; t.w[i][w + 2] = v.z; t.w[i][w + 3] = v.w;
             } else if constexpr (A::VP == 2) {
-                const uint2 v = load_stream(reinterpret_cast<const uint2 *>(piece));
+                const uint2 v = *reinterpret_cast<const uint2 *>(piece);
                 t.w[i][w] = v.x; t.w[i][w + 1] = v.y;
             } else {
-                t.w[i][w] = load_stream(reinterpret_cast<const uint32_t *>(piece));
+                t.w[i][w] = *reinterpret_cast<const uint32_t *>(piece);
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) load_scales<TYPE, D>(t.d[i], kv.v_scale, row0 + r + 8 * i);
+    for (int i = 0; i < 2; ++i) load_scales<TYPE, D>(t.d[i], tile + B::VS, r + 8 * i);
 }
 
 // Operand A of the score product's k step: 16 keys by 16 head_dim indexes.  Lane column c's values v = 0, 1 (of the first 8 columns) and 2, 3 (of
@@ -303,7 +343,11 @@ struct AttnShape {
     static constexpr int MIN_BLOCKS = D <= 128 && NT == 1 && !(F32 && BF) ? 3 : 1;    // to an SM: 168 registers
     static constexpr int ROWS = 8 * NT;
     static constexpr int Q_WORDS = QT * STEPS * NT * 64;
-    static constexpr size_t SMEM_Q = Q_WORDS * 4 + ROWS * 8;                       // operands, then factor and reach of every row
+    static constexpr int PASS_BYTES = KS * TileBytes<TYPE, D>::ALL;
+    static constexpr int STAGES = PASS_BYTES <= 5120 ? 3 : 2;                      // passes in a warp's ring
+    static constexpr size_t RING = Q_WORDS * 4 + ROWS * 8;                         // where the rings begin: behind the operands, factor and reach of every row
+    static constexpr size_t SMEM_Q = RING + ATTN_WARPS * STAGES * PASS_BYTES;
+    static_assert(RING % 16 == 0 && PASS_BYTES % 16 == 0, "16-byte pieces");
     static constexpr size_t SMEM_O = (size_t) ATTN_WARPS * ROWS * (D + 2) * 4;     // outputs, maxima and sums of the warps
     static constexpr size_t SMEM = SMEM_Q > SMEM_O ? SMEM_Q : SMEM_O;
 };
@@ -352,30 +396,37 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
     auto place = [&](int key) { return key < front ? key : key - front; };
     auto tile_page = [&](int key) { return key < key_end ? (key < front ? p.prefix_pages : table)[place(key) >> shift] : 0; };
     auto tile_row = [&](int page, int key) { return (((int64_t) page * p.kv.n_head + head) << shift) + (place(key) & in_page); };
-    KeyRegs<TYPE, D> kr[S::KS];
-    ValueRegs<TYPE, D> vr[S::KS];
-    int page[S::KS], next_page[S::KS];
-    bool good[S::KS];
-    int key = key0 + warp * 16 * S::KS;
+    uint8_t * ring = reinterpret_cast<uint8_t *>(smem) + S::RING + warp * (S::STAGES * S::PASS_BYTES);
+    int page[S::KS];       // of the pass that is copied next
+    uint32_t there = 0;    // tiles of the ring whose page is there, a bit to stage and tile
+    auto fill = [&](int stage, int key) {
+        if (key < key_end) {
 #pragma unroll
-    for (int j = 0; j < S::KS; ++j) page[j] = tile_page(key + 16 * j);
-#pragma unroll
-    for (int j = 0; j < S::KS; ++j) next_page[j] = tile_page(key + STRIDE + 16 * j);
-    auto check = [&](int j) {
-        good[j] = page[j] >= 0 && page[j] < n_pages;
-        if (!good[j]) {
-            if (lane == 0) report_error(p.err, DEV_ERR_BAD_SLOT);
-            page[j] = 0;
+            for (int j = 0; j < S::KS; ++j) {
+                const bool good = page[j] >= 0 && page[j] < n_pages;
+                const uint32_t bit = 1u << (stage * S::KS + j);
+                there = good ? there | bit : there & ~bit;
+                if (!good && lane == 0) report_error(p.err, DEV_ERR_BAD_SLOT);
+                fill_tile<TYPE, D>(ring + stage * S::PASS_BYTES + j * TileBytes<TYPE, D>::ALL, p.kv, tile_row(good ? page[j] : 0, key + 16 * j), lane);
+            }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (key < key_end) {
+    int key = key0 + warp * 16 * S::KS;
+    {
+        int first_pages[S::STAGES][S::KS];
 #pragma unroll
-        for (int j = 0; j < S::KS; ++j) {
-            check(j);
-            const int64_t row = tile_row(page[j], key + 16 * j);
-            load_keys<TYPE, D>(kr[j], p.kv, row, lane);
-            load_values<TYPE, D>(vr[j], p.kv, row, lane);
+        for (int i = 0; i < S::STAGES; ++i)
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j) first_pages[i][j] = tile_page(key + i * STRIDE + 16 * j);
+#pragma unroll
+        for (int i = 0; i < S::STAGES; ++i) {
+#pragma unroll
+            for (int j = 0; j < S::KS; ++j) page[j] = first_pages[i][j];
+            fill(i, key + i * STRIDE);
         }
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) page[j] = tile_page(key + S::STAGES * STRIDE + 16 * j);
     }
     // ---- the queries as operands, eight values to a thread at a time; the first keys and values are on their way
     {
@@ -451,7 +502,14 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[t][n][i] = 0.0f;
 
+    int stage = 0;
     for (; key < key_end; key += STRIDE) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 1) : "memory");
+        __syncwarp();    // all lanes' copies of this pass are there
+        const uint8_t * tiles = ring + stage * S::PASS_BYTES;
+        KeyRegs<TYPE, D> kr[S::KS];
+#pragma unroll
+        for (int j = 0; j < S::KS; ++j) load_keys<TYPE, D>(kr[j], tiles + j * TileBytes<TYPE, D>::ALL, lane);
         // ---- scores: 16 keys by 8 NT rows; lane has keys r, r + 8 and rows 2c, 2c + 1
         float s[S::KS][NT][4];
 #pragma unroll
@@ -495,25 +553,15 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
                         s[j][n][i] = TYPE == KV_BF16 ? s[j][n][i] + part[j][n][i] : fmaf(part[j][n][i], kr[j].d[i >> 1][g], s[j][n][i]);
         }
         bool masked = key + 16 * S::KS > seen_by_all || key + 16 * S::KS > key_end || (key < front && key + 16 * S::KS > p.own_prefix);
-#pragma unroll
-        for (int j = 0; j < S::KS; ++j) masked |= !good[j];
         bool was_good[S::KS];
 #pragma unroll
-        for (int j = 0; j < S::KS; ++j) was_good[j] = good[j];
-        // ---- the next keys fly from here on
-        const int next = key + STRIDE;
-#pragma unroll
         for (int j = 0; j < S::KS; ++j) {
-            page[j] = next_page[j];
-            next_page[j] = tile_page(next + STRIDE + 16 * j);
+            was_good[j] = there >> (stage * S::KS + j) & 1;
+            masked |= !was_good[j];
         }
-        if (next < key_end) {
+        ValueRegs<TYPE, D> vr[S::KS];
 #pragma unroll
-            for (int j = 0; j < S::KS; ++j) {
-                check(j);
-                load_keys<TYPE, D>(kr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
-            }
-        }
+        for (int j = 0; j < S::KS; ++j) load_values<TYPE, D>(vr[j], tiles + j * TileBytes<TYPE, D>::ALL, lane);
         // ---- softmax and outputs; the form for tiles that some row does not see in full costs a third more
         auto weigh = [&](auto form) {
             constexpr bool MASKED = decltype(form)::value;
@@ -689,11 +737,15 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
         };
         if (masked) weigh(std::true_type{});
         else weigh(std::false_type{});
-        if (next < key_end) {
+        // the pass is used up: its place takes the one that follows those on their way
+        __syncwarp();
+        const int next = key + S::STAGES * STRIDE;
+        fill(stage, next);
 #pragma unroll
-            for (int j = 0; j < S::KS; ++j) load_values<TYPE, D>(vr[j], p.kv, tile_row(page[j], next + 16 * j), lane);
-        }
+        for (int j = 0; j < S::KS; ++j) page[j] = tile_page(next + STRIDE + 16 * j);
+        if (++stage == S::STAGES) stage = 0;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 
     // ---- join the warps
     if (!PREFIX) pdl_launch_dependents();

@@ -182,8 +182,8 @@ int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn
 int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int n_head, int n_tokens, bool f32, AttnPlan & pl) {
     const int group = n_head / c->n_head_kv, most = attend_tiles(c->head_dim, f32);
     const int pass = 32 * ATTN_WARPS;
-    // about one wave of blocks (three to an SM) where all are as long, two where sequences are not and short ones make room for long ones
-    const int64_t one_wave = (int64_t) ctx->sm_count * 3, blocks = a->n_seq > 1 ? 2 * one_wave : one_wave;
+    // about one wave of blocks (three to an SM) where all are as long, three where sequences are not and short ones make room for long ones
+    const int64_t one_wave = (int64_t) ctx->sm_count * 3, blocks = a->n_seq > 1 ? 3 * one_wave : one_wave;
     pl = AttnPlan{};
     const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
     const bool own_tc = !f32 && own_rows >= ATTN_TC_ROWS, prefix_tc = !f32 && rows >= ATTN_TC_ROWS;
