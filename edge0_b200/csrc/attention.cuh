@@ -803,8 +803,13 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
         if (p.direct || (!PREFIX && p.cluster)) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             XT * dst = reinterpret_cast<XT *>(p.out + (int64_t) token * p.out_token + (int64_t) h * p.out_head) + d;
-            dst[0] = from_float<XT>(x * inv);
-            dst[1] = from_float<XT>(y * inv);
+            const Pack<XT, 2> v = { { from_float<XT>(x * inv), from_float<XT>(y * inv) } };
+            if (p.out_aligned) {
+                *reinterpret_cast<Pack<XT, 2> *>(dst) = v;
+            } else {
+                dst[0] = v.v[0];
+                dst[1] = v.v[1];
+            }
             if (p.lse && d == 0) p.lse[line] = sum == 0.0f ? -INFINITY : (most + log2f(sum)) * 0.69314718055994531f;
         } else {
             *reinterpret_cast<float2 *>(p.part_o + (line * chunks + slot) * D + d) = make_float2(x, y);

@@ -270,13 +270,23 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
         return clean && !finite ? __uint_as_float(0x7fffffffu) : pow2_inverse(up);
     } else {
         const uint32_t w[4] = { t.v[n].x, t.v[n].y, t.v[n].z, t.v[n].w };
-        uint32_t top = 0;
+        // sizes as bf16 bits, two to a word; what is not finite says nothing about the others' size
+        uint32_t top = 0, bad = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t size = w[i] & 0x7fff7fffu, off = __vcmpgeu2(size, 0x7f807f80u);
+            top = __vmaxu2(top, size & ~off);
+            bad |= off;
+        }
 #pragma unroll
-        for (int o = S::TPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float up = row_up(top);
-        const bool zero = clean && top >= 0x7f800000u;    // the whole row: its weights become NaN
+        for (int o = S::TPR / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float up = row_up(max(top << 16, top & 0xffff0000u));
+        bool zero = false;    // the whole row: its weights become NaN
+        if (VALUES && clean) {    // the same for the whole block
+#pragma unroll
+            for (int o = S::TPR / 2; o > 0; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+            zero = bad != 0;
+        }
         uint32_t h[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)

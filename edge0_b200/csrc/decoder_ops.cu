@@ -135,6 +135,9 @@ struct AttnPlan {
 };
 
 constexpr int64_t WALK_BYTES = 8 << 20;
+// Fewest keys that a block is started for, where there are as many (64 sequences of up to 512 keys behind a prefix: 44.6 us with 128, 40.5 with 256,
+// 41.1 with 512).
+constexpr int LEAST_KEYS = 256;
 // Most keys to a block of a cluster.
 constexpr int CLUSTER_KEYS = 1024;
 // Up to so many chunks a row is joined by one warp.
@@ -145,9 +148,9 @@ constexpr int TC_TILE = 0;     // nt of those kernels, whose tile goes by the he
 
 int tile_units(int64_t rows, int most) { return rows <= 8 ? 1 : rows <= 16 ? 2 : most; }
 
-// keys to a chunk, a multiple of `unit`, so that `base` blocks of whole length become about `blocks`
-void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int & chunk, int & chunks) {
-    const int64_t n = std::max<int64_t>(1, std::min({ (len + unit - 1) / unit, blocks / std::max<int64_t>(base, 1), (int64_t) JOIN_CHUNKS / 2 }));
+// keys to a chunk, a multiple of `unit` and `least` or more where there are as many, so that `base` blocks of whole length become about `blocks`
+void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int least, int & chunk, int & chunks) {
+    const int64_t n = std::max<int64_t>(1, std::min({ (len + least - 1) / least, blocks / std::max<int64_t>(base, 1), (int64_t) JOIN_CHUNKS / 2 }));
     chunk = (int) std::max<int64_t>(unit, ((len + n - 1) / n + unit - 1) / unit * unit);
     chunks = (int) ((len + chunk - 1) / chunk);
 }
@@ -155,9 +158,10 @@ void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int & chunk
 // The same for the kernels with tiles of many rows, one block to an SM: the number of chunks whose waves take least, in tiles of 64 keys.  A block
 // costs about three tiles beside its keys (queries in, outputs out), and the join about four.
 void split_keys_tc(int64_t len, int64_t base, int64_t sms, int & chunk, int & chunks) {
-    const int64_t tiles = std::max<int64_t>(1, (len + 63) / 64);
-    int64_t best = INT64_MAX, n_best = 1;
-    for (int64_t n = 1; n <= std::min<int64_t>(tiles, 64); ++n) {
+    const int tiles = (int) std::max<int64_t>(1, (len + 63) / 64);
+    int64_t best = INT64_MAX;
+    int n_best = 1;
+    for (int n = 1; n <= std::min(tiles, 64) && (n == 1 || base * n <= 4 * sms); ++n) {    // beyond four waves more chunks do not help
         const int64_t cost = (base * n + sms - 1) / sms * ((tiles + n - 1) / n + 3) + (n > 1 ? 4 : 0);
         if (cost < best) { best = cost; n_best = n; }
     }
@@ -187,28 +191,28 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     pl = AttnPlan{};
     const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
     const bool own_tc = !f32 && own_rows >= ATTN_TC_ROWS, prefix_tc = !f32 && rows >= ATTN_TC_ROWS;
-    // sequences that fill tiles of their own walk the prefix themselves: the products take the same time, and nothing is left to join
-    if (a->prefix_len && own_tc && own_rows >= 128) pl.own_prefix = a->prefix_len;
     pl.own_nt = own_tc ? TC_TILE : tile_units(own_rows, most);
     auto tiles = [&](int64_t n, int nt) { const int tile = nt == TC_TILE ? attend_tc_rows(c->head_dim) : 8 * nt; return (int) ((n + tile - 1) / tile); };
     pl.own_tiles = tiles(own_rows, pl.own_nt);
     const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles;
     // A prefix is walked by every sequence, too, where that reads little twice: the launches and the join that it saves take as long as about 8 MB of
-    // the cache (56 heads, two sequences of 23 keys behind 31: 13.8 us with a launch of its own, 5.8 walked).
-    const int64_t again = (int64_t) a->prefix_len * (a->n_seq - 1) * c->n_head_kv * 2 * row_bytes(c->type, c->head_dim);
-    if (a->prefix_len && !own_tc && (again <= WALK_BYTES || (int64_t) a->prefix_len * (a->n_seq - 1) <= (int64_t) a->n_seq * a->max_kv_len / 4)) pl.own_prefix = a->prefix_len;
+    // the cache (56 heads, two sequences of 23 keys behind 31: 13.8 us with a launch of its own, 5.8 walked).  Sequences that fill a group's 128 rows by
+    // themselves walk it in any case: the products take the same time, and nothing is left to join.
+    const int64_t again = (int64_t) a->prefix_len * std::max(a->n_seq - 1, 0), own_keys = (int64_t) a->n_seq * a->max_kv_len;
+    const int64_t row = (int64_t) c->n_head_kv * 2 * row_bytes(c->type, c->head_dim);
+    if (a->prefix_len && ((own_tc && own_rows >= 128) || again * row <= WALK_BYTES || again <= own_keys / 4)) pl.own_prefix = a->prefix_len;
     pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
     const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
     if (own_tc) {
         split_keys_tc(own_len, own_base, ctx->sm_count, pl.own_chunk, pl.own_chunks);
     } else {
-        split_keys(own_len, own_base, blocks, pass, pl.own_chunk, pl.own_chunks);
+        split_keys(own_len, own_base, blocks, pass, LEAST_KEYS, pl.own_chunk, pl.own_chunks);
         // Few blocks: clusters of chunks that join themselves, while all of them are resident together and a block has not too many keys
         const int64_t most_blocks = (c->head_dim == 256 || (f32 && c->type == KV_BF16 && c->head_dim == 128) ? 2 : 3) * (int64_t) ctx->sm_count;
         if (pl.own_chunks > 1 && (pl.own_prefix || !a->prefix_len)) {
-            const int64_t n = std::min<int64_t>({ ATTN_CLUSTER, most_blocks / std::max<int64_t>(own_base, 1), pl.own_chunks });
+            const int64_t n = std::min<int64_t>({ c->head_dim == 256 ? 8 : ATTN_CLUSTER, most_blocks / std::max<int64_t>(own_base, 1), pl.own_chunks });
             if (n > 1 && (own_len + n - 1) / n <= CLUSTER_KEYS) {
-                split_keys(own_len, 1, n, pass, pl.own_chunk, pl.own_chunks);
+                split_keys(own_len, 1, n, pass, pass, pl.own_chunk, pl.own_chunks);
                 pl.cluster = pl.own_chunks > 1;
             }
         }
@@ -219,7 +223,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
         pl.prefix_tiles = tiles(rows, pl.prefix_nt);
         const int64_t base = (int64_t) c->n_head_kv * pl.prefix_tiles;
         if (prefix_tc) split_keys_tc(a->prefix_len, base, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
-        else split_keys(a->prefix_len, base, one_wave, pass, pl.prefix_chunk, pl.prefix_chunks);
+        else split_keys(a->prefix_len, base, one_wave, pass, LEAST_KEYS, pl.prefix_chunk, pl.prefix_chunks);
     }
     if ((int64_t) pl.own_tiles * pl.own_chunks > INT32_MAX || (int64_t) pl.prefix_tiles * pl.prefix_chunks > INT32_MAX)
         return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
@@ -349,11 +353,12 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     if (!elem_size(x_type)) return fail(ctx, B200MOE_ERR_UNSUPPORTED, "q must be F32 or BF16");
     if (!q || !out || !a) return fail(ctx, B200MOE_ERR_INVALID_ARG, "null argument");
     if (int rc = check_attn(ctx, cache, a, q->ne[1], q->ne[2])) return rc;
-    if (q->ne[2] == 0 || a->n_seq == 0 || a->max_new == 0) return B200MOE_OK;
+    if (q->ne[2] == 0 || a->n_seq == 0 || (a->q_start && a->max_new == 0)) return B200MOE_OK;
     if (int rc = check_rows(ctx, q, x_type, "q", false)) return rc;
     if (int rc = check_rows(ctx, out, x_type, "out", true)) return rc;
     for (int i = 0; i < 3; ++i) if (q->ne[i] != out->ne[i]) return fail(ctx, B200MOE_ERR_INVALID_ARG, "q and out differ in shape");
     if (q->ne[0] != cache->head_dim) return fail(ctx, B200MOE_ERR_INVALID_ARG, "q has another head_dim than the cache");
+    if (!a->q_start && a->max_new != 1) return fail(ctx, B200MOE_ERR_INVALID_ARG, "without q_start every sequence has one new token: max_new must be 1");
     if (!a->q_start && q->ne[2] < a->n_seq) return fail(ctx, B200MOE_ERR_INVALID_ARG, "fewer tokens than sequences");
     if (!a->kv_len || (a->max_kv_len && !a->pages) || (a->prefix_len && !a->prefix_pages)) return fail(ctx, B200MOE_ERR_INVALID_ARG, "null lengths or pages");
     const bool f32 = x_type == B200MOE_TYPE_F32;
@@ -367,7 +372,7 @@ int b200moe_attention(b200moe_ctx * c, const b200moe_kv_cache * cache, const b20
     p.lse = lse;
     p.q_head = q->nb[1]; p.q_token = q->nb[2]; p.out_head = out->nb[1]; p.out_token = out->nb[2];
     p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / cache->n_head_kv;
-    p.n_seq = a->n_seq; p.max_new = a->q_start ? a->max_new : 1; p.max_kv_len = a->max_kv_len; p.prefix_len = a->prefix_len; p.pages_stride = a->pages_stride;
+    p.n_seq = a->n_seq; p.max_new = a->max_new; p.max_kv_len = a->max_kv_len; p.prefix_len = a->prefix_len; p.pages_stride = a->pages_stride;
     p.q_start = a->q_start; p.kv_len = a->kv_len; p.pages = a->pages; p.prefix_pages = a->prefix_pages;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.own_chunk = pl.own_chunk; p.own_chunks = pl.own_chunks;

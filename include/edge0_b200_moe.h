@@ -395,7 +395,7 @@ B200MOE_API int b200moe_kv_read(b200moe_ctx * ctx, const b200moe_kv_cache * cach
  * F32: everything to fp32's accuracy (weights in steps of 2^-38 of the largest). */
 typedef struct b200moe_attn {
     int32_t n_seq;
-    int32_t max_new;                 /* most new tokens of a sequence */
+    int32_t max_new;                 /* most new tokens of a sequence (1 without q_start) */
     int32_t max_kv_len;              /* most positions of a sequence, at most pages_stride * page_size */
     int32_t prefix_len;              /* 0: no prefix */
     int32_t pages_stride;            /* entries of `pages` from one sequence to the next */

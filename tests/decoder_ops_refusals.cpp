@@ -137,7 +137,10 @@ int main() {
     ATTEND(PASSED, );
     ATTEND(OK, q.ne[2] = o.ne[2] = 0);
     ATTEND(OK, a.n_seq = 0);
-    ATTEND(OK, a.max_new = 0);
+    ATTEND(OK, a.max_new = 0, a.q_start = ints);
+    ATTEND(ARG, a.max_new = 0);
+    ATTEND(ARG, a.max_new = 2);
+    ATTEND(PASSED, a.max_new = 2, a.q_start = ints);
     ATTEND(ARG, a.n_seq = -1);
     ATTEND(ARG, a.max_new = -1);
     ATTEND(ARG, a.prefix_len = -1);

@@ -266,6 +266,45 @@ def test_nan_within_reach_is_seen(gpu_ctx, kind):
     assert torch.isnan(b.call()[:, G:]).all() and torch.isfinite(b.call()[:, :G]).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("what", ["inf", "nan"])
+def test_the_other_columns_of_a_row_with_an_infinity(gpu_ctx, kind, what):
+    """A value that is not finite spoils outputs of its head only; in a BF16 cache, where a row has no scale, its own column alone (or, where some token
+    does not see the key, the head), and never another value's share."""
+    for n_head, new in ((8, None), (256, None), (8, [40, 40])):
+        b = Batch(gpu_ctx, kind, [300, 90], new=new, n_head=n_head, n_kv=2, prefix=64)
+        clean, _, tol = b.expected()
+        G = n_head // 2
+        x = b.v[(b.prefix_pages[1] * b.page + 2).long()][None].clone()
+        x[0, 1, 5] = float(what)
+        b.cache.write(b.k[(b.prefix_pages[1] * b.page + 2).long()][None].contiguous(), x, (b.prefix_pages[1] * b.page + 2).to(torch.int32).reshape(1))
+        out = b.call()
+        assert ((out[:, :G].double() - clean[:, :G]).abs() <= tol[:, :G]).all()
+        assert not torch.isfinite(out[:, G:, 5]).any()
+        rest = torch.ones(b.D, dtype=torch.bool, device="cuda")
+        rest[{"bf16": slice(5, 6), "q8": slice(0, b.D), "q4": slice(0, 32)}[kind]] = False
+        got, want, bound = out[:, G:, rest].double(), clean[:, G:, rest], tol[:, G:, rest]
+        assert ((got - want).abs() <= bound).logical_or(torch.isnan(got)).all()
+        if new is None:
+            assert torch.isfinite(got).all()
+    gpu_ctx.synchronize()
+
+
+def test_many_rows_behind_the_last_sequence(gpu_ctx):
+    for prefix in (0, 3000):
+        b = Batch(gpu_ctx, "q4", [130, 200], new=[20, 31], prefix=prefix)
+        want, _, tol = b.expected()
+        q = torch.cat([b.q, torch.full((9, b.n_head, b.D), float("nan"), dtype=b.dtype, device="cuda")])
+        out = torch.full_like(q, 3.0)
+        b.call(q=q, out=out)
+        assert ((out[:51].double() - want).abs() <= tol).all() and (out[51:] == 3).all()
+        out.fill_(3.0)
+        b.call(q=q, out=out, kv_len=torch.tensor([130, 201], dtype=torch.int32, device="cuda"))
+        with pytest.raises(B200MoeError, match="code 5"):
+            gpu_ctx.synchronize()
+        assert ((out[:20].double() - want[:20]).abs() <= tol[:20]).all() and (out[20:] == 3).all()
+
+
 def test_rows_behind_the_last_sequence_and_bad_lengths(gpu_ctx):
     b = Batch(gpu_ctx, "q8", [30, 200], new=[2, 3], prefix=50)
     b.check()
@@ -433,6 +472,12 @@ def test_refusals(gpu_ctx):
         b.call(out=b.q[:1])
     with pytest.raises(TypeError):
         b.call(q=b.q.half())
+    with pytest.raises(ValueError):
+        b.call(q=b.q.cpu())
+    with pytest.raises(ValueError):
+        b.call(kv_len=b.kv_len.cpu())
+    with pytest.raises(B200MoeError):
+        b.call(q_start=None, max_new=2)
     with pytest.raises(B200MoeError):
         b.call(q=b.q[:, :65])
     with pytest.raises(B200MoeError):

@@ -151,5 +151,9 @@ def test_graph_stream_and_empty(gpu_ctx):
         gpu_ctx.rope(x, pos.long())
     with pytest.raises(ValueError):
         gpu_ctx.rope(x, pos[:3])
+    with pytest.raises(ValueError):
+        gpu_ctx.rope(x.cpu(), pos)
+    with pytest.raises(ValueError):
+        gpu_ctx.rope(x, pos.cpu())
     with pytest.raises(TypeError):
         gpu_ctx.rope(x.half(), pos)
