@@ -304,7 +304,6 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
     uint8_t * sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t) 1023);
     uint8_t * sk = sq + GROUPS * S::Q_BYTES, * sv = sk + NS * S::KV_BYTES;
     __shared__ uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS];
-    __shared__ uint64_t turn[2][4];    // [group][warp of the group]: its turn at the exponentials
     __shared__ uint64_t q_full, s_full[2 * GROUPS], p_full[2 * GROUPS], pv_done[2 * GROUPS];    // [group][parity of the tile]
     __shared__ __align__(16) float k_scale[NS][KT], v_scale[NS][KT];
     __shared__ float s_factor[GROUPS * TC_GROUP_ROWS];
@@ -346,7 +345,6 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             mbar_init(&p_full[i], TC_GROUP_ROWS);
             mbar_init(&pv_done[i], 1);
         }
-        for (int i = 0; i < 8; ++i) mbar_init(&turn[i / 4][i % 4], 1);
         mbar_init(&q_full, 32 * SW);
         mbar_fence_init();
         s_abort = 0;
@@ -502,12 +500,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                         }
                     }
                 }
-                // The weights, over the scores.  The two groups' warps of a scheduler take turns here: together they would wait for the exponentials at
-                // the same time and for everything else at the same time, too (a tile 3,000 cycles, MEASURED in turns).
-                if (n_groups == 2) {
-                    ok = __all_sync(0xffffffffu, wait_suspended(&turn[group][warp & 3], group == 0 ? (i & 1) ^ 1u : i & 1, &s_abort, p.err));
-                    if (!ok) break;
-                }
+                // the weights, over the scores
                 const float base = ref == -INFINITY ? 0.0f : -ref;
                 const uint64_t base2 = pack2(base, base), factor2 = pack2(factor, factor);
                 if (!masked) {
@@ -537,7 +530,6 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                         s[0][c / 2] = half2_bits(__floats2half2_rn(v[0], v[1]));
                     }
                 }
-                if (n_groups == 2 && lane == 0) mbar_arrive(&turn[group ^ 1][warp & 3]);
                 tmem_store32(t_s, s[0]);
                 tmem_wait_st();
                 tc_fence_before();
