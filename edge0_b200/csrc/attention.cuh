@@ -863,14 +863,25 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
 constexpr int JOIN_THREADS = 256, JOIN_CHUNKS = 1024;
 template <int D, typename XT, int WARPS>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ AttnParams p) {
-    constexpr int PER = D / 32, LINES = JOIN_THREADS / 32 / WARPS, MOST = WARPS == 1 ? 32 : JOIN_CHUNKS;
+    constexpr int PER = D / 32, LINES = JOIN_THREADS / 32 / WARPS, MOST = WARPS == 1 ? 32 : JOIN_CHUNKS, AHEAD = WARPS == 1 ? 8 : 1;
     __shared__ float s_weight[LINES][MOST];
     __shared__ float s_sum[WARPS], s_most[WARPS];
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = WARPS == 1 ? warp : 0, part = WARPS == 1 ? 0 : warp;
     const int64_t line = (int64_t) blockIdx.x * LINES + sub;
     if (line >= (int64_t) p.n_tokens * p.n_head) return;    // whole warps, of which none waits for another (LINES is 1 where they do)
-    const int token = (int) (line / p.n_head);
+    const int token = (int) (line / p.n_head), chunks = p.prefix_chunks + p.own_chunks;
+    const float2 * ml = p.part_ml + line * chunks;
+    const float * o = p.part_o + line * chunks * D;
+    // One warp to a row: its loads are on their way before it is known how many chunks the row has; what no chunk wrote is not looked at
+    Pack<float, PER> ahead[AHEAD];
+    float2 mine = make_float2(-INFINITY, 0.0f);
+    if (WARPS == 1) {
+        if (lane < chunks) mine = ml[lane];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (i < chunks) ahead[i] = *reinterpret_cast<const Pack<float, PER> *>(o + (int64_t) i * D + lane * PER);
+    }
     int seq = token;
     if (p.q_start) {    // the last sequence that begins at or before the token
         int low = 0, high = p.n_seq;
@@ -885,12 +896,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
     if (seq >= p.n_seq || !attn_sequence(p, seq, first, n_new, len, false) || token < first || token >= first + n_new) return;    // a row that belongs to nobody
     const int reach = p.own_front + max(0, len - n_new + (token - first) + 1);
     const int own = (reach + p.own_chunk - 1) / p.own_chunk;
-    const int n = p.prefix_chunks + own, chunks = p.prefix_chunks + p.own_chunks;
-    const float2 * ml = p.part_ml + line * chunks;
-    const float * o = p.part_o + line * chunks * D;
+    const int n = p.prefix_chunks + own;
     // ---- the chunks' weights
     float most = -INFINITY, sum = 0.0f;
-    for (int i = part * 32 + lane; i < n; i += 32 * WARPS) most = fmaxf(most, ml[i].x);
+    for (int i = part * 32 + lane; i < n; i += 32 * WARPS) most = fmaxf(most, WARPS == 1 ? mine.x : ml[i].x);
 #pragma unroll
     for (int x = 16; x > 0; x /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
     if (WARPS > 1) {
@@ -900,7 +909,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
         for (int w = 0; w < WARPS; ++w) most = fmaxf(most, s_most[w]);
     }
     for (int i = part * 32 + lane; i < n; i += 32 * WARPS) {
-        const float2 x = ml[i];
+        const float2 x = WARPS == 1 ? mine : ml[i];
         const float f = x.x == -INFINITY ? 0.0f : fast_exp2(x.x - most);
         const bool some = x.x != -INFINITY || x.y != 0.0f;
         s_weight[sub][i] = some ? f : -1.0f;    // nothing there: the outputs are not to be looked at
@@ -921,8 +930,17 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_
     float acc[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
+    if (WARPS == 1) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (i < n) {
+                const float f = s_weight[sub][i];
+#pragma unroll
+                for (int j = 0; j < PER; ++j) acc[j] += f < 0.0f ? 0.0f : ahead[i].v[j] * f;
+            }
+    }
 #pragma unroll 8
-    for (int i = part; i < n; i += WARPS) {
+    for (int i = WARPS == 1 ? AHEAD : part; i < n; i += WARPS) {
         const Pack<float, PER> v = *reinterpret_cast<const Pack<float, PER> *>(o + (int64_t) i * D + lane * PER);
         const float f = s_weight[sub][i];
 #pragma unroll
