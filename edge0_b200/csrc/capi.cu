@@ -1295,12 +1295,16 @@ int b200moe_create(int device, b200moe_ctx ** out) {
     if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) { cudaGetLastError(); return B200MOE_ERR_NO_DEVICE; }
     if (device < 0 || device >= n) return B200MOE_ERR_INVALID_ARG;
     if (cudaSetDevice(device) != cudaSuccess) { cudaGetLastError(); return B200MOE_ERR_CUDA; }
-    cudaDeviceProp prop{};
-    if (cudaGetDeviceProperties(&prop, device) != cudaSuccess) { cudaGetLastError(); return B200MOE_ERR_CUDA; }
-    if (prop.major != 10) return B200MOE_ERR_UNSUPPORTED;  // kernels are built for sm_100a only
+    int major = 0, sms = 0;    // two attributes: all properties of a device take milliseconds to gather
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        cudaGetLastError();
+        return B200MOE_ERR_CUDA;
+    }
+    if (major != 10) return B200MOE_ERR_UNSUPPORTED;  // kernels are built for sm_100a only
     auto * ctx = new b200moe_ctx();
     ctx->device = device;
-    ctx->sm_count = prop.multiProcessorCount;
+    ctx->sm_count = sms;
     if (cudaMalloc(&ctx->d_err, 16) != cudaSuccess || cudaMemset(ctx->d_err, 0, 16) != cudaSuccess ||
         cudaMallocHost(&ctx->h_err, 16) != cudaSuccess) {
         cudaGetLastError();
