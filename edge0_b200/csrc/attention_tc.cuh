@@ -336,13 +336,13 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
         for (int i = 0; i < NS; ++i) {
             mbar_init(&k_full[i], 32 * TC_PRODUCER_WARPS);
             mbar_init(&v_full[i], 32 * TC_PRODUCER_WARPS);
-            mbar_init(&k_free[i], 5 * n_groups);    // a commit and four softmax warps of each group
-            mbar_init(&v_free[i], 5 * n_groups);
+            mbar_init(&k_free[i], n_groups);    // commits
+            mbar_init(&v_free[i], n_groups);
             s_bad[i] = 0;
         }
         for (int i = 0; i < 2 * GROUPS; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], TC_GROUP_ROWS);
+            mbar_init(&p_full[i], 4);    // warps
             mbar_init(&pv_done[i], 1);
         }
         mbar_init(&q_full, 32 * SW);
@@ -427,11 +427,9 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                 const uint32_t t_s = t_lane + S::T_S + b * KT;
                 // the votes reconverge the warp and make the outcome uniform for the instructions that need all of it
                 bool ready = mbar_try_wait(&s_full[b], b_ph);
-                ready &= mbar_try_wait(&k_full[st], ph);
                 ready &= mbar_try_wait(&v_full[st], ph);
                 if (!__all_sync(0xffffffffu, ready)) {
-                    ok = __all_sync(0xffffffffu, wait_suspended(&s_full[b], b_ph, &s_abort, p.err) && wait_suspended(&k_full[st], ph, &s_abort, p.err) &&
-                                                     wait_suspended(&v_full[st], ph, &s_abort, p.err));
+                    ok = __all_sync(0xffffffffu, wait_suspended(&s_full[b], b_ph, &s_abort, p.err) && wait_suspended(&v_full[st], ph, &s_abort, p.err));
                     if (!ok) break;
                 }
                 tc_fence_after();
@@ -533,12 +531,8 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                 tmem_store32(t_s, s[0]);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[b]);
                 __syncwarp();
-                if (lane == 0) {    // the tile's factors have been read
-                    mbar_arrive(&k_free[st]);
-                    mbar_arrive(&v_free[st]);
-                }
+                if (lane == 0) mbar_arrive(&p_full[b]);    // the tile's factors have been read, too
             }
             // ---- the outputs
             const int last = n_tiles - 1;
@@ -650,12 +644,10 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             const bool masked = masked_tile(i, 0);
             const int to = in_tile * S::NL * S::ROWS + r0;
             if (in_tile == 0 && !__all_sync(0xffffffffu, wait_suspended(&k_free[st], ph ^ 1u, &s_abort, p.err))) break;
+            float k_factor[S::NL];
 #pragma unroll
-            for (int n = 0; n < S::NL; ++n) {
-                const float f = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, false);
-                if (x == 0) k_scale[st][to + n * S::ROWS] = gone >> n & 1 ? -1.0f : there >> n & 1 ? f : 0.0f;
-            }
-            if (gone) s_bad[st] = i + 1;
+            for (int n = 0; n < S::NL; ++n)
+                k_factor[n] = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, false);
             if (in_tile == S::PARTS - 1) {
                 fence_async_smem();
                 mbar_arrive(&k_full[st]);
@@ -664,11 +656,16 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                 find(part + 1);
                 tc_load<TYPE, D>(k, p.kv.k, p.kv.k_scale, p.kv, slot, head, x);
             }
+            // the factors of both lie with the values: what frees those came after the weights, for which they were read
             if (in_tile == 0 && !__all_sync(0xffffffffu, wait_suspended(&v_free[st], ph ^ 1u, &s_abort, p.err))) break;
+            if (gone) s_bad[st] = i + 1;
 #pragma unroll
             for (int n = 0; n < S::NL; ++n) {
                 const float f = tc_store<TYPE, D, true>(v, n, sv + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, masked);
-                if (x == 0) v_scale[st][to + n * S::ROWS] = there >> n & 1 ? f : 0.0f;
+                if (x == 0) {
+                    k_scale[st][to + n * S::ROWS] = gone >> n & 1 ? -1.0f : there >> n & 1 ? k_factor[n] : 0.0f;
+                    v_scale[st][to + n * S::ROWS] = there >> n & 1 ? f : 0.0f;
+                }
                 top = fmaxf(top, there >> n & 1 ? f : 0.0f);    // not a number: says nothing here, makes the weight one
             }
             if (in_tile == S::PARTS - 1) {
