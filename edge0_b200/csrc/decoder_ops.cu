@@ -155,14 +155,18 @@ void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int least, 
     chunks = (int) ((len + chunk - 1) / chunk);
 }
 
-// The same for the kernels with tiles of many rows, one block to an SM: the number of chunks whose waves take least, in tiles of 64 keys.  A block
-// costs about three tiles beside its keys (queries in, outputs out), and the join about four.
-void split_keys_tc(int64_t len, int64_t base, int64_t sms, int & chunk, int & chunks) {
+// The same for the kernels with tiles of many rows, one block to an SM: the number of chunks that takes least, in tiles of 64 keys.  A block costs
+// about five tiles beside its keys (queries in, outputs out), the join about four.  Blocks of one length come in whole waves.  Of several sequences'
+// about three quarters have keys (lengths are known on the device alone), and long and short ones fill an SM's time between them: counted as whole
+// waves, all of them full, eight sequences of 500 .. 2000 keys and 64 new tokens took 51.1 us (two chunks) for 43.0 (three), four of 1000 .. 3000
+// and 128 new ones 53.7 (two) for 44.8 (three).
+void split_keys_tc(int64_t len, int64_t base, bool ragged, int64_t sms, int & chunk, int & chunks) {
     const int tiles = (int) std::max<int64_t>(1, (len + 63) / 64);
     int64_t best = INT64_MAX;
     int n_best = 1;
     for (int n = 1; n <= std::min(tiles, 64) && (n == 1 || base * n <= 4 * sms); ++n) {    // beyond four waves more chunks do not help
-        const int64_t cost = (base * n + sms - 1) / sms * ((tiles + n - 1) / n + 3) + (n > 1 ? 4 : 0);
+        const int64_t turns = ragged ? std::max(sms, base * n * 3 / 4) : (base * n + sms - 1) / sms * sms;    // SMs' times for a block
+        const int64_t cost = turns * ((tiles + n - 1) / n + 5) + (n > 1 ? 4 * sms : 0);
         if (cost < best) { best = cost; n_best = n; }
     }
     chunk = (int) ((tiles + n_best - 1) / n_best * 64);
@@ -204,7 +208,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
     const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
     if (own_tc) {
-        split_keys_tc(own_len, own_base, ctx->sm_count, pl.own_chunk, pl.own_chunks);
+        split_keys_tc(own_len, own_base, a->n_seq > 1, ctx->sm_count, pl.own_chunk, pl.own_chunks);
     } else {
         split_keys(own_len, own_base, blocks, pass, LEAST_KEYS, pl.own_chunk, pl.own_chunks);
         // Few blocks: clusters of chunks that join themselves, while all of them are resident together and a block has not too many keys
@@ -222,7 +226,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
         pl.prefix_nt = prefix_tc ? TC_TILE : tile_units(rows, most);
         pl.prefix_tiles = tiles(rows, pl.prefix_nt);
         const int64_t base = (int64_t) c->n_head_kv * pl.prefix_tiles;
-        if (prefix_tc) split_keys_tc(a->prefix_len, base, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
+        if (prefix_tc) split_keys_tc(a->prefix_len, base, false, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
         else split_keys(a->prefix_len, base, one_wave, pass, LEAST_KEYS, pl.prefix_chunk, pl.prefix_chunks);
     }
     if ((int64_t) pl.own_tiles * pl.own_chunks > INT32_MAX || (int64_t) pl.prefix_tiles * pl.prefix_chunks > INT32_MAX)
