@@ -11,14 +11,19 @@
 //                        An instruction holds its thread about 75 cycles whatever its size, and a commit more: one thread for all took
 //                        3,300 cycles to a tile.  Every group has two buffers of scores, so that the next tile's are ready when a tile's softmax ends
 //
-// Precision.  Every operand is f16 and every factor a power of two or outside: rows of Q and of BF16 and Q4 caches are brought to the same size by a power of
-// two a row (bf16's 8 bits, and a 3-bit code times an 8-bit scale, fit f16's 11), Q8 codes are whole numbers; a key's factor multiplies its score,
-// a value's its weight, in fp32.  The weights 2^(s - ref) times the values' factors are rounded to f16 (2^-11).  ref rises only when a tile's
+// Precision.  A BF16 cache's scores are bf16 products, its keys and the queries as they are.  Every other operand is f16 and every factor a power of two
+// or outside: rows of Q, of Q4 caches and of BF16 values are brought to the same size by a power of two a row (bf16's 8 bits, and a 3-bit
+// code times an 8-bit scale, fit f16's 11), Q8 codes are whole numbers; a key's factor multiplies its score, a value's its weight, in fp32.  The weights 2^(s - ref) times the values' factors are rounded to f16 (2^-11).  ref rises only when a tile's
 // maximum is more than 2^8 above it: weights stay below 2^15, sums are fp32.
 //
-// Bound by the exponentials (16 a cycle and SM: 1,024 cycles for 64 keys of 256 rows), the products (about 1,200 cycles with operands read
-// from shared memory at 128 bytes a cycle) and issue (a score costs about five instructions, packed fp32 pairs where there are such; a value of
-// the cache 1.2 (Q8) to 2.5 (BF16), shared by the block's 256 rows).
+// Measured (32 query and 4 key/value heads of 128, Q8): 64 sequences behind 8192 shared keys 40 us in all, 512 new tokens on 4096 keys 77 us
+// (420 TFLOP/s), two and three times as fast as the kernel of few rows.  A tile of 64 keys and 256 rows takes about 2,900 cycles (2,400
+// once the producers are done), the products alone 1,024, the exponentials (16 a cycle and SM) as many: a scheduler has two softmax warps, a
+// producer and an issuer, each of which gets an instruction through every sixth cycle (issue 40 %; a score costs about five instructions,
+// packed fp32 pairs where there are such, a value of the cache 1.2 (Q8) to 2.5 (BF16), shared by the block's 256 rows).  Beside its keys a
+// block spends some 9,000 cycles before the first scores and 7,000 on the outputs.  Slower were: two threads to a row (16 softmax warps of 80
+// registers: 93 us for the 77, the producers starve), producers of keys and of values apart (65 us for 62 on chunks of three prompts),
+// groups that take turns at the exponentials (65 for 62).
 #pragma once
 #include "attention.cuh"
 #include "tensor_core.cuh"
@@ -268,6 +273,9 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
             *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, 4 * (run * GB + g) + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         return clean && !finite ? __uint_as_float(0x7fffffffu) : pow2_inverse(up);
+    } else if (!VALUES) {    // bf16 products: as they are
+        *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, x)) = t.v[n];
+        return 1.0f;
     } else {
         const uint32_t w[4] = { t.v[n].x, t.v[n].y, t.v[n].z, t.v[n].w };
         // sizes as bf16 bits, two to a word; what is not finite says nothing about the others' size
@@ -282,7 +290,7 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
         for (int o = S::TPR / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float up = row_up(max(top << 16, top & 0xffff0000u));
         bool zero = false;    // the whole row: its weights become NaN
-        if (VALUES && clean) {    // the same for the whole block
+        if (clean) {    // the same for the whole block
 #pragma unroll
             for (int o = S::TPR / 2; o > 0; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
             zero = bad != 0;
@@ -396,6 +404,13 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             for (int n = 0; n < BATCH; ++n) {
                 const int row = r0 + n * PASS + tid / TPR;
                 const uint32_t w[4] = { raw[n].x, raw[n].y, raw[n].z, raw[n].w };
+                uint8_t * to = sq + (row / TC_GROUP_ROWS) * S::Q_BYTES + tc_offset(TC_GROUP_ROWS, row % TC_GROUP_ROWS, x);
+                if (TYPE == KV_BF16) {
+                    const uint32_t flip = sign < 0.0f ? 0x80008000u : 0u;
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
+                    if (x == 0) s_factor[row] = fabsf(p.scale_log2);
+                    continue;
+                }
                 // sizes as bf16 bits, two to a word: they have the numbers' order
                 uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
@@ -405,7 +420,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     h2[i] = half2_bits(__floats2half2_rn(__uint_as_float(w[i] << 16) * (up * sign), __uint_as_float(w[i] & 0xffff0000u) * (up * sign)));
-                *reinterpret_cast<uint4 *>(sq + (row / TC_GROUP_ROWS) * S::Q_BYTES + tc_offset(TC_GROUP_ROWS, row % TC_GROUP_ROWS, x)) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(h2[0], h2[1], h2[2], h2[3]);
                 if (x == 0) s_factor[row] = fabsf(p.scale_log2) * pow2_inverse(up);
             }
         }
@@ -457,6 +472,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
                         }
                 }
                 tmem_wait_ld();
+                if (TYPE != KV_BF16)    // whose keys have no factors
 #pragma unroll
                 for (int c = 0; c < KT; c += 4) {
                     const float4 f = ks[c / 4];
@@ -682,7 +698,8 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
         const int g = (warp - SW - TC_PRODUCER_WARPS) >> 1;
         const bool outputs = (warp - SW - TC_PRODUCER_WARPS) & 1;
         if (g < n_groups && !outputs) {
-            constexpr uint32_t IDESC = (1u << 4) | ((uint32_t) (KT >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t BF16 = TYPE == KV_BF16 ? 1u << 7 | 1u << 10 : 0u;    // both operands; else f16
+            constexpr uint32_t IDESC = (1u << 4) | BF16 | ((uint32_t) (KT >> 3) << 17) | ((128u >> 4) << 24);
             const uint32_t a = smem_u32(sq) + g * S::Q_BYTES;
             const bool queries = wait_suspended(&q_full, 0, &s_abort, p.err);
             for (int i = 0; i < n_tiles && queries; ++i) {
