@@ -134,16 +134,26 @@ struct AttnPlan {
     size_t part_o, bytes;
 };
 
-constexpr int64_t WALK_BYTES = 8 << 20;
+// A prefix may be walked by every sequence for itself, in place of a launch for all rows and a join, up to so many keys read again, times head_dim and
+// the square of the key/value heads: the more heads, the more a walked key costs, and the more blocks a launch of its own has to be fast
+// with.  Q8, heads of 128, up to 512 own keys, walked and with a launch of its own: 4 heads, 64 sequences behind 256 keys 20 us and 29,
+// behind 512 23 and 26, behind 1024 30 and 28 (bf16 22 and 38, 25 and 29, 34 and 32); 8 heads, 64 sequences behind 256 24 and 36, 16 behind
+// 2048 27 and 25; 32 heads, two sequences behind 1024 11 and 14, behind 2048 19 and 16; 66 heads, two behind 256 11 and 11, behind 1024 19 and 16.
+constexpr int64_t WALK_KEYS = 160 << 20;
 // Fewest keys that a block is started for, where there are as many (64 sequences of up to 512 keys behind a prefix: 44.6 us with 128, 40.5 with 256,
 // 41.1 with 512).
 constexpr int LEAST_KEYS = 256;
-// Most keys to a block of a cluster.
-constexpr int CLUSTER_KEYS = 1024;
-// Up to so many chunks a row is joined by one warp.
+// Most keys to a block of a cluster (one sequence, bf16: 4096 keys 8.4 us, joined through the workspace 10.4; with blocks of up to 1024 keys 16384
+// were 17.0 for 13.2, four sequences of up to 16384 29.2 for 24.6).
+constexpr int CLUSTER_KEYS = 256;
+// Up to so many chunks a row is joined by one warp, which is all that a block of eight joins else (chunks of three prompts 59.7 us and 87.9, a
+// batch of 64 40.8 and 44.6).
 constexpr int JOIN_FEW = 32;
-// From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries).
-constexpr int ATTN_TC_ROWS = 64;
+// From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries); for a prefix, whose rows are the whole batch's, from more
+// than half as many.  8192 keys, Q8: 64 rows 24.1 us and 25.6 with the kernel of few rows, 128 rows 24.1 and 48.8; 16 sequences of up to
+// 4096 with 64 rows 49 and 64.  bf16, where values cost more to bring into f16: 96 rows 29.3 and 27.3, 128 rows 29.5 and 50.3.  A prefix of
+// 16000, Q8: 32 rows 28 and 27, 48 rows 29 and 48; 8192, bf16: 64 rows 29 and 29, 128 rows 30 and 53.
+constexpr int attn_tc_rows(int type) { return type == KV_BF16 ? 128 : 64; }
 constexpr int TC_TILE = 0;     // nt of those kernels, whose tile goes by the head_dim
 
 int tile_units(int64_t rows, int most) { return rows <= 8 ? 1 : rows <= 16 ? 2 : most; }
@@ -157,7 +167,7 @@ void split_keys(int64_t len, int64_t base, int64_t blocks, int unit, int least, 
 
 // The same for the kernels with tiles of many rows, one block to an SM: the number of chunks that takes least, in tiles of 64 keys.  A block costs
 // about five tiles beside its keys (queries in, outputs out), the join about four.  Blocks of one length come in whole waves.  Of several sequences'
-// about three quarters have keys (lengths are known on the device alone), and long and short ones fill an SM's time between them: counted as whole
+// about four in five have keys (lengths are known on the device alone), and long and short ones fill an SM's time between them: counted as whole
 // waves, all of them full, eight sequences of 500 .. 2000 keys and 64 new tokens took 51.1 us (two chunks) for 43.0 (three), four of 1000 .. 3000
 // and 128 new ones 53.7 (two) for 44.8 (three).
 void split_keys_tc(int64_t len, int64_t base, bool ragged, int64_t sms, int & chunk, int & chunks) {
@@ -165,7 +175,10 @@ void split_keys_tc(int64_t len, int64_t base, bool ragged, int64_t sms, int & ch
     int64_t best = INT64_MAX;
     int n_best = 1;
     for (int n = 1; n <= std::min(tiles, 64) && (n == 1 || base * n <= 4 * sms); ++n) {    // beyond four waves more chunks do not help
-        const int64_t turns = ragged ? std::max(sms, base * n * 3 / 4) : (base * n + sms - 1) / sms * sms;    // SMs' times for a block
+        const int64_t typical = base * n * 4 / 5;
+        // SMs' times for a block; a second wave that has but a few blocks is not free (two sequences of 4000 and 8000 keys and 8 new tokens: 35.8 us in
+        // 152 blocks, 27.3 in 128)
+        const int64_t turns = !ragged ? (base * n + sms - 1) / sms * sms : typical <= sms ? sms : typical + sms / 16;
         const int64_t cost = turns * ((tiles + n - 1) / n + 5) + (n > 1 ? 4 * sms : 0);
         if (cost < best) { best = cost; n_best = n; }
     }
@@ -194,17 +207,17 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     const int64_t one_wave = (int64_t) ctx->sm_count * 3, blocks = a->n_seq > 1 ? 3 * one_wave : one_wave;
     pl = AttnPlan{};
     const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
-    const bool own_tc = !f32 && own_rows >= ATTN_TC_ROWS, prefix_tc = !f32 && rows >= ATTN_TC_ROWS;
+    const int tc_rows = attn_tc_rows(c->type);
+    const bool own_tc = !f32 && own_rows >= tc_rows, prefix_tc = !f32 && rows > tc_rows / 2;
     pl.own_nt = own_tc ? TC_TILE : tile_units(own_rows, most);
     auto tiles = [&](int64_t n, int nt) { const int tile = nt == TC_TILE ? attend_tc_rows(c->head_dim) : 8 * nt; return (int) ((n + tile - 1) / tile); };
     pl.own_tiles = tiles(own_rows, pl.own_nt);
     const int64_t own_base = (int64_t) a->n_seq * c->n_head_kv * pl.own_tiles;
-    // A prefix is walked by every sequence, too, where that reads little twice: the launches and the join that it saves take as long as about 8 MB of
-    // the cache (56 heads, two sequences of 23 keys behind 31: 13.8 us with a launch of its own, 5.8 walked).  Sequences that fill a group's 128 rows by
-    // themselves walk it in any case: the products take the same time, and nothing is left to join.
+    // A prefix is walked by every sequence where that reads little twice, or little beside the own keys (56 heads, two sequences of 23 keys behind 31: 13.8 us
+    // with a launch of its own, 5.8 walked; 64 sequences of up to 4000 keys behind 1024: 59.9 and 45.8).  Sequences that fill a group's 128 rows
+    // by themselves walk it in any case: the products take the same time, and nothing is left to join.
     const int64_t again = (int64_t) a->prefix_len * std::max(a->n_seq - 1, 0), own_keys = (int64_t) a->n_seq * a->max_kv_len;
-    const int64_t row = (int64_t) c->n_head_kv * 2 * row_bytes(c->type, c->head_dim);
-    if (a->prefix_len && ((own_tc && own_rows >= 128) || again * row <= WALK_BYTES || again <= own_keys / 4)) pl.own_prefix = a->prefix_len;
+    if (a->prefix_len && ((own_tc && own_rows >= 128) || again * c->n_head_kv * c->head_dim <= WALK_KEYS / c->n_head_kv || again <= own_keys / 4)) pl.own_prefix = a->prefix_len;
     pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
     const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
     if (own_tc) {

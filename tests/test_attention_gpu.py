@@ -487,3 +487,52 @@ def test_refusals(gpu_ctx):
     with pytest.raises(ValueError):
         b.call(lse=torch.empty(3, device="cuda"))
     gpu_ctx.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prefix_of_a_wide_batch(gpu_ctx, kind, D, dtype):
+    """Prefixes too long to be walked by every sequence: few rows to a key/value head, and many, of which some are nobody's."""
+    Batch(gpu_ctx, kind, [5, 90, 1, 44, 0], prefix=2077, n_head=40, n_kv=20, D=D, dtype=dtype, seed=1).check()
+    Batch(gpu_ctx, kind, [5, 70, 1] * 11, prefix=5003, n_head=32, n_kv=8, D=D, dtype=dtype, seed=2, page=64).check()
+    b = Batch(gpu_ctx, kind, [9, 33] * 20, new=[3, 2] * 20, prefix=1200, n_head=28, n_kv=14, D=D, dtype=dtype, seed=3, page=32)
+    b.check()
+    want, _, tol = b.expected()
+    q = torch.cat([b.q, torch.full((7, b.n_head, D), float("nan"), dtype=dtype, device="cuda")])
+    out = torch.full_like(q, 3.0)
+    b.call(q=q, out=out)
+    assert ((out[:b.T].double() - want).abs() <= tol).all() and (out[b.T:] == 3).all()
+    b.ctx.synchronize()
+
+
+def test_many_rows_replayed_on_two_streams(gpu_ctx):
+    """Graphs of the tensor-memory kernels side by side, lengths and tables changed between replays."""
+    cases = [Batch(gpu_ctx, kind, [300, 170], new=[40, 40], n_head=16, n_kv=2, prefix=prefix, seed=7) for kind, prefix in (("bf16", 0), ("q8", 90), ("q4", 5000))]
+    graphs, outs = [], []
+    for x in cases:
+        out = torch.zeros_like(x.q)
+        x.call(out=out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            x.call(out=out)
+        graphs.append(g)
+        outs.append(out)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for step, lens in enumerate(([300, 170], [41, 40], [0, 299], [256, 64])):
+        for x, o in zip(cases, outs):
+            x.lens = [min(n, 16 * x.pages.shape[1]) for n in lens]
+            x.kv_len.copy_(torch.tensor(x.lens, dtype=torch.int32))
+            x.q.copy_(torch.randn(x.q.shape, generator=torch.Generator().manual_seed(step)).to(x.dtype))
+            o.fill_(5.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for x, o in zip(cases, outs):
+            want, _, tol = x.expected()
+            assert ((o.double() - want).abs() <= tol).all()
+    gpu_ctx.synchronize()
