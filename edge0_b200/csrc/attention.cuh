@@ -15,6 +15,12 @@
 // before are worked on (two thirds of what 227 KB hold is in flight; a register's worth ahead, as before, was 48 KB an SM and 2.9 TB/s); no barrier in
 // the loop.  Pieces of a row lie at piece ^ swizzle(row), so that both kinds of reads meet no bank conflicts on rows of 128 bytes and more.
 //
+// Measured (32 query and 4 key/value heads of 128): 64 sequences of 200 .. 4096 keys, Q8, 41 us (3.6 TB/s of cache; 55 % of what a copy moves), one
+// of 131072, Q4, 34 us, one of 4096, bf16, 8 us.  Q8 and Q4 are bound by issue: some 460 instructions to a pass of 16 keys of a warp, 2.6
+// warps to a scheduler (the outputs' and operands' 140 .. 154 registers allow three blocks), which issues in half of the cycles;
+// bf16 decode of a large batch reaches 80 % of a copy's rate.  Small calls are bound by the latency of two or three dependent reads
+// (lengths, pages, rows) and the join.
+//
 // Precision.  The codes are whole numbers and go into the product exactly; the scales stay outside in fp32: a key's multiplies the score,
 // a value's the weight p.  Q8 and Q4: codes as f16 (a byte or nibble under the exponent of 1024), queries as f16 with a power of two to a row that
 // puts its largest value at 2^14 (bf16 queries lose nothing that is above 2^-28 of the row's largest; fp32 ones are split in two), weights times scales
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
         ValueRegs<TYPE, D> vr[S::KS];
 #pragma unroll
         for (int j = 0; j < S::KS; ++j) load_values<TYPE, D>(vr[j], tiles + j * TileBytes<TYPE, D>::ALL, lane);
-        // ---- softmax and outputs; the form for tiles that some row does not see in full costs a third more
+        // ---- softmax and outputs; tiles that some row does not see in full have a form of their own
         auto weigh = [&](auto form) {
             constexpr bool MASKED = decltype(form)::value;
             bool on[S::KS][NT][4];
@@ -858,8 +864,8 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
 }
 
 // Joins the chunks of a (token, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c.  WARPS warps to a row: one where there are few chunks,
-// eight with their loads in flight together where a long axis was cut into many (a document of 131072 keys, 205 chunks: 30 us with
-// four warps that each read a chunk's maximum before its outputs, 6 now).
+// eight with their loads in flight together where a long axis was cut into many (a document of 131072 keys, 103 chunks: the whole
+// call takes 34 us; with four warps that each read a chunk's maximum before its outputs the join alone took 30).
 constexpr int JOIN_THREADS = 256, JOIN_CHUNKS = 1024;
 template <int D, typename XT, int WARPS>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const __grid_constant__ AttnParams p) {
