@@ -174,7 +174,8 @@ void split_keys_tc(int64_t len, int64_t base, bool ragged, int64_t sms, int & ch
     const int tiles = (int) std::max<int64_t>(1, (len + 63) / 64);
     int64_t best = INT64_MAX;
     int n_best = 1;
-    for (int n = 1; n <= std::min(tiles, 64) && (n == 1 || base * n <= 4 * sms); ++n) {    // beyond four waves more chunks do not help
+    const int most = (int) std::min<int64_t>(std::min(tiles, 64), 4 * sms / std::max<int64_t>(base, 1));    // beyond four waves more chunks do not help
+    for (int n = 1; n <= most; ++n) {
         const int64_t typical = base * n * 4 / 5;
         // SMs' times for a block; a second wave that has but a few blocks is not free (two sequences of 4000 and 8000 keys and 8 new tokens: 35.8 us in
         // 152 blocks, 27.3 in 128)
@@ -217,7 +218,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     // with a launch of its own, 5.8 walked; 64 sequences of up to 4000 keys behind 1024: 59.9 and 45.8).  Sequences that fill a group's 128 rows
     // by themselves walk it in any case: the products take the same time, and nothing is left to join.
     const int64_t again = (int64_t) a->prefix_len * std::max(a->n_seq - 1, 0), own_keys = (int64_t) a->n_seq * a->max_kv_len;
-    if (a->prefix_len && ((own_tc && own_rows >= 128) || again * c->n_head_kv * c->head_dim <= WALK_KEYS / c->n_head_kv || again <= own_keys / 4)) pl.own_prefix = a->prefix_len;
+    if (a->prefix_len && ((own_tc && own_rows >= 128) || again <= WALK_KEYS / ((int64_t) c->n_head_kv * c->n_head_kv * c->head_dim) || again <= own_keys / 4)) pl.own_prefix = a->prefix_len;
     pl.own_front = own_tc ? pl.own_prefix : (pl.own_prefix + 15) / 16 * 16;
     const int64_t own_len = (int64_t) a->max_kv_len + pl.own_front;
     if (own_tc) {

@@ -10,8 +10,8 @@
 //
 // Bound by memory: every value is read and written once.  2305 tokens of 32 + 4 heads of 128 (bf16) take 10 us, 55 % of a copy's rate
 // with cold caches, the launch, the positions and the sines in it; a single token takes 2.8 us.  A block takes a few tokens, works out their
-// pairs' sines and cosines once into shared memory (a table entry serves every head of the token) and then runs over the heads with 16-byte loads and stores; rows or strides
-// that are not multiples of 16 bytes go pair by pair.
+// pairs' sines and cosines once into shared memory (a table entry serves every head of the token) and then runs over the heads with 16-byte
+// loads and stores; rows or strides that are not multiples of 16 bytes go pair by pair.
 #pragma once
 #include <cuda_bf16.h>
 
