@@ -12,9 +12,10 @@
 //                        3,300 cycles to a tile.  Every group has two buffers of scores, so that the next tile's are ready when a tile's softmax ends
 //
 // Precision.  A BF16 cache's scores are bf16 products, its keys and the queries as they are.  Every other operand is f16 and every factor a power of two
-// or outside: rows of Q, of Q4 caches and of BF16 values are brought to the same size by a power of two a row (bf16's 8 bits, and a 3-bit
-// code times an 8-bit scale, fit f16's 11), Q8 codes are whole numbers; a key's factor multiplies its score, a value's its weight, in fp32.  The weights 2^(s - ref) times the values' factors are rounded to f16 (2^-11).  ref rises only when a tile's
-// maximum is more than 2^8 above it: weights stay below 2^15, sums are fp32.
+// or outside: rows of Q and of Q4 caches and BF16 values, a row or a warp's rows together, are brought to the same size by a power of two (bf16's 8 bits,
+// and a 3-bit code times an 8-bit scale, fit f16's 11), Q8 codes are whole numbers; a key's factor multiplies its score, a value's its weight, in
+// fp32.  The weights 2^(s - ref) times the values' factors are rounded to f16 (2^-11).  ref rises only when a tile's maximum is more than
+// 2^8 above it: weights stay below 2^15, sums are fp32.
 //
 // Measured (32 query and 4 key/value heads of 128, Q8): 64 sequences behind 8192 shared keys 40 us in all, 512 new tokens on 4096 keys 77 us
 // (420 TFLOP/s), two and three times as fast as the kernel of few rows.  A tile of 64 keys and 256 rows takes about 2,900 cycles (2,400
@@ -178,7 +179,7 @@ __device__ __forceinline__ uint64_t umma_desc_v(uint32_t smem_addr, uint32_t blo
 
 // 2^(14 - e) for the largest exponent field e among a row's values, and the power that undoes it; kept where both are normal
 __device__ __forceinline__ float row_up(uint32_t amax_bits) {
-    const int e = min(max((int) (amax_bits >> 23), 40), 250);
+    const int e = min(max((int) (amax_bits >> 23), 40), 254);
     return __uint_as_float((uint32_t) (254 + 14 - e) << 23);
 }
 __device__ __forceinline__ float pow2_inverse(float p) { return __uint_as_float((254u << 23) - __float_as_uint(p)); }
@@ -208,9 +209,33 @@ __device__ __forceinline__ void tc_load(TcPiece<TYPE, D> & t, const uint8_t * ro
     }
 }
 
+// The power of two for a BF16 cache's values in a tile that every query sees: one for all rows that a warp holds, by the largest of them that is finite.
+// It costs no more than the steps of the weights do, which go by the largest value, too: f16 keeps what is above 2^-28 of that in full and
+// steps of 2^-38 below.
+template <int TYPE, int D>
+__device__ __forceinline__ float tc_values_up(const TcPiece<TYPE, D> & t) {
+    auto most = [&](bool finite) {    // sizes as bf16 bits, two to a word
+        uint32_t top = 0;
+#pragma unroll
+        for (int n = 0; n < TcShape<TYPE, D>::NL; ++n) {
+            const uint32_t w[4] = { t.v[n].x, t.v[n].y, t.v[n].z, t.v[n].w };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t size = w[i] & 0x7fff7fffu;
+                top = __vmaxu2(top, finite ? size & ~__vcmpgeu2(size, 0x7f807f80u) : size);
+            }
+        }
+        return __reduce_max_sync(0xffffffffu, max(top << 16, top & 0xffff0000u));
+    };
+    uint32_t top = most(false);
+    if (top >= 0x7f800000u) top = most(true);
+    return row_up(top);
+}
+
 // converts a row's 16 bytes and stores them; returns the row's factor.  clean: values that are not finite are stored as zeros and the factor is NaN.
+// up: tc_values_up for a BF16 cache's values, not looked at where `clean`.
 template <int TYPE, int D, bool VALUES>
-__device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uint8_t * tile, int row, int x, bool there, bool clean) {
+__device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uint8_t * tile, int row, int x, bool there, bool clean, float up) {
     typedef TcShape<TYPE, D> S;
     if (TYPE == KV_Q8) {
         uint4 lo, hi;
@@ -242,7 +267,7 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
             finite &= ok;
             if (ok) top = max(top, d[g]);
         }
-        const float up = row_up(top) * 0.125f;
+        const float scale_up = row_up(top) * 0.125f;
         const int run = x / (D >= 128 ? 4 : 2), in_run = D >= 128 ? x % 4 : x;
         const uint32_t w[4] = { t.v[n].x, t.v[n].y, t.v[n].z, t.v[n].w };
 #pragma unroll
@@ -260,7 +285,7 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
 #pragma unroll
             for (int j = 0; j < G; ++j) if (j == run * GB + g) scale = __uint_as_float(d[j]);
             const bool zero = !there || (clean && !(scale < INFINITY));
-            const __half2 s2 = __float2half2_rn(scale * up);
+            const __half2 s2 = __float2half2_rn(scale * scale_up);
             const uint32_t even = q & 0x0f0f0f0fu, odd = (q >> 4) & 0x0f0f0f0fu;
             const uint32_t a = __byte_perm(even, odd, 0x5140), b = __byte_perm(even, odd, 0x7362);    // nibbles 0 1 2 3, 4 5 6 7
             uint32_t h[4];
@@ -272,27 +297,27 @@ __device__ __forceinline__ float tc_store(const TcPiece<TYPE, D> & t, int n, uin
             }
             *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, 4 * (run * GB + g) + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
-        return clean && !finite ? __uint_as_float(0x7fffffffu) : pow2_inverse(up);
+        return clean && !finite ? __uint_as_float(0x7fffffffu) : pow2_inverse(scale_up);
     } else if (!VALUES) {    // bf16 products: as they are
         *reinterpret_cast<uint4 *>(tile + tc_offset(TC_KEYS, row, x)) = t.v[n];
         return 1.0f;
     } else {
         const uint32_t w[4] = { t.v[n].x, t.v[n].y, t.v[n].z, t.v[n].w };
-        // sizes as bf16 bits, two to a word; what is not finite says nothing about the others' size
-        uint32_t top = 0, bad = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t size = w[i] & 0x7fff7fffu, off = __vcmpgeu2(size, 0x7f807f80u);
-            top = __vmaxu2(top, size & ~off);
-            bad |= off;
-        }
-#pragma unroll
-        for (int o = S::TPR / 2; o > 0; o >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float up = row_up(max(top << 16, top & 0xffff0000u));
         bool zero = false;    // the whole row: its weights become NaN
-        if (clean) {    // the same for the whole block
+        if (clean) {          // the same for the whole block; some queries see a part of the tile: each row by its own size
+            uint32_t top = 0, bad = 0;
 #pragma unroll
-            for (int o = S::TPR / 2; o > 0; o >>= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t size = w[i] & 0x7fff7fffu, off = __vcmpgeu2(size, 0x7f807f80u);
+                top = __vmaxu2(top, size & ~off);
+                bad |= off;
+            }
+#pragma unroll
+            for (int o = S::TPR / 2; o > 0; o >>= 1) {
+                top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+            }
+            up = row_up(max(top << 16, top & 0xffff0000u));
             zero = bad != 0;
         }
         uint32_t h[4];
@@ -663,7 +688,7 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             float k_factor[S::NL];
 #pragma unroll
             for (int n = 0; n < S::NL; ++n)
-                k_factor[n] = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, false);
+                k_factor[n] = tc_store<TYPE, D, false>(k, n, sk + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, false, 1.0f);
             if (in_tile == S::PARTS - 1) {
                 fence_async_smem();
                 mbar_arrive(&k_full[st]);
@@ -675,9 +700,10 @@ __global__ void __launch_bounds__(TcShape<TYPE, D>::THREADS, 1) attend_tc_kernel
             // the factors of both lie with the values: what frees those came after the weights, for which they were read
             if (in_tile == 0 && !__all_sync(0xffffffffu, wait_suspended(&v_free[st], ph ^ 1u, &s_abort, p.err))) break;
             if (gone) s_bad[st] = i + 1;
+            const float up = TYPE == KV_BF16 && !masked ? tc_values_up<TYPE, D>(v) : 1.0f;
 #pragma unroll
             for (int n = 0; n < S::NL; ++n) {
-                const float f = tc_store<TYPE, D, true>(v, n, sv + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, masked);
+                const float f = tc_store<TYPE, D, true>(v, n, sv + st * S::KV_BYTES, to + n * S::ROWS, x, there >> n & 1, masked, up);
                 if (x == 0) {
                     k_scale[st][to + n * S::ROWS] = gone >> n & 1 ? -1.0f : there >> n & 1 ? k_factor[n] : 0.0f;
                     v_scale[st][to + n * S::ROWS] = there >> n & 1 ? f : 0.0f;

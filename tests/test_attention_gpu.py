@@ -536,3 +536,24 @@ def test_many_rows_replayed_on_two_streams(gpu_ctx):
             want, _, tol = x.expected()
             assert ((o.double() - want).abs() <= tol).all()
     gpu_ctx.synchronize()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("what", ["nan", "inf", "3e38"])
+def test_many_rows_and_what_they_do_not_see(gpu_ctx, kind, what):
+    """New tokens of a chunk see nothing of those behind them, be they infinite, not numbers or merely large."""
+    b = Batch(gpu_ctx, kind, [250, 77, 64], new=[70, 77, 40], prefix=45)
+    clean = b.check()
+    tail = [3, 60, 40]    # of each sequence's new tokens are replaced
+    slots = torch.cat([b.pages[s].repeat_interleave(b.page)[n - m:n] * b.page + torch.arange(n - m, n, device="cuda") % b.page
+                       for s, (n, m) in enumerate(zip(b.lens, tail))]).to(torch.int32)
+    x = torch.full((sum(tail), b.n_kv, b.D), float(what), dtype=torch.bfloat16, device="cuda")
+    b.cache.write(x, x, slots)
+    out = b.call()
+    at = [0, 70, 147]
+    before = torch.cat([torch.arange(a, a + n - m) for a, n, m in zip(at, b.new, tail)]).cuda()
+    assert torch.equal(out[before], clean[before])
+    if what != "3e38":
+        behind = torch.tensor([t for t in range(b.T) if t not in set(before.tolist())], device="cuda")
+        assert not torch.isfinite(out[behind]).any()
+    b.ctx.synchronize()
