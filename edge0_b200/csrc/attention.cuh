@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(32 * ATTN_WARPS, (AttnShape<TYPE, D, XT, NT>::
                 for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[n][j]));
 #pragma unroll
                 for (int o = TPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const int e = min(max((int) (__float_as_uint(m) >> 23), 40), 250);    // 2^(e - 127) <= m, kept where both powers are normal
+                const int e = min(max((int) (__float_as_uint(m) >> 23), 40), 254);    // 2^(e - 127) <= m, kept where both powers are normal
                 up = __uint_as_float((uint32_t) (254 + 14 - e) << 23);
                 factor = p.scale_log2 / up;
             }

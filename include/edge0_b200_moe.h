@@ -391,6 +391,7 @@ B200MOE_API int b200moe_kv_read(b200moe_ctx * ctx, const b200moe_kv_cache * cach
  * reports like a page that the cache does not have (its positions count as unseen).  What lies in the cache behind a sequence's length, or
  * a token's reach, has no influence, whatever it is; an infinity or NaN within reach makes outputs infinite or NaN.
  * lse (or NULL): F32 [n_head, tokens], the natural logarithm of the sum of exp(scale * q . k_j), -inf where there are no positions.
+ * Over a BF16 cache q . k_j itself has to be in fp32's range, before the scale.
  * BF16 queries: products of the held values in full, weights rounded to f16 (2^-11 of each, and steps of 2^-31 of the largest) or finer;
  * F32: everything to fp32's accuracy (weights in steps of 2^-38 of the largest). */
 typedef struct b200moe_attn {

@@ -557,3 +557,10 @@ def test_many_rows_and_what_they_do_not_see(gpu_ctx, kind, what):
         behind = torch.tensor([t for t in range(b.T) if t not in set(before.tolist())], device="cuda")
         assert not torch.isfinite(out[behind]).any()
     b.ctx.synchronize()
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [None, [80, 70]])
+def test_queries_near_the_largest_number(gpu_ctx, kind, dtype, new):
+    Batch(gpu_ctx, kind, [300, 90], new=new, dtype=dtype, loud=6e37).check(scale=128 ** -0.5 / 6e37)
