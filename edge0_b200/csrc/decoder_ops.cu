@@ -204,8 +204,13 @@ int check_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn
 int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn * a, int n_head, int n_tokens, bool f32, AttnPlan & pl) {
     const int group = n_head / c->n_head_kv, most = attend_tiles(c->head_dim, f32);
     const int pass = 32 * ATTN_WARPS;
-    // about one wave of blocks (three to an SM) where all are as long, three where sequences are not and short ones make room for long ones
-    const int64_t one_wave = (int64_t) ctx->sm_count * 3, blocks = a->n_seq > 1 ? 3 * one_wave : one_wave;
+    // about one wave of blocks where all are as long, three where sequences are not and short ones make room for long ones; registers leave three
+    // blocks to an SM, or two (bf16 cache, cut for two and for three: one sequence of 8192 keys with 96 rows 29 us and 41, 56 rows behind a prefix of
+    // 16000 35 and 50; fp32 queries 22 and 34, 34 and 47)
+    auto one_wave = [&](int nt) {
+        const bool two = c->head_dim == 256 || nt == 4 || (c->head_dim == 128 && (nt == 2 || (f32 && c->type == KV_BF16)));
+        return (int64_t) ctx->sm_count * (two ? 2 : 3);
+    };
     pl = AttnPlan{};
     const int64_t own_rows = (int64_t) std::min(a->max_new, n_tokens) * group, rows = (int64_t) n_tokens * group;
     const int tc_rows = attn_tc_rows(c->type);
@@ -224,11 +229,11 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
     if (own_tc) {
         split_keys_tc(own_len, own_base, a->n_seq > 1, ctx->sm_count, pl.own_chunk, pl.own_chunks);
     } else {
-        split_keys(own_len, own_base, blocks, pass, LEAST_KEYS, pl.own_chunk, pl.own_chunks);
+        const int64_t wave = one_wave(pl.own_nt);
+        split_keys(own_len, own_base, a->n_seq > 1 ? 3 * wave : wave, pass, LEAST_KEYS, pl.own_chunk, pl.own_chunks);
         // Few blocks: clusters of chunks that join themselves, while all of them are resident together and a block has not too many keys
-        const int64_t most_blocks = (c->head_dim == 256 || (f32 && c->type == KV_BF16 && c->head_dim == 128) ? 2 : 3) * (int64_t) ctx->sm_count;
         if (pl.own_chunks > 1 && (pl.own_prefix || !a->prefix_len)) {
-            const int64_t n = std::min<int64_t>({ c->head_dim == 256 ? 8 : ATTN_CLUSTER, most_blocks / std::max<int64_t>(own_base, 1), pl.own_chunks });
+            const int64_t n = std::min<int64_t>({ c->head_dim == 256 ? 8 : ATTN_CLUSTER, wave / std::max<int64_t>(own_base, 1), pl.own_chunks });
             if (n > 1 && (own_len + n - 1) / n <= CLUSTER_KEYS) {
                 split_keys(own_len, 1, n, pass, pass, pl.own_chunk, pl.own_chunks);
                 pl.cluster = pl.own_chunks > 1;
@@ -241,7 +246,7 @@ int plan_attn(ContextBase * ctx, const b200moe_kv_cache * c, const b200moe_attn 
         pl.prefix_tiles = tiles(rows, pl.prefix_nt);
         const int64_t base = (int64_t) c->n_head_kv * pl.prefix_tiles;
         if (prefix_tc) split_keys_tc(a->prefix_len, base, false, ctx->sm_count, pl.prefix_chunk, pl.prefix_chunks);
-        else split_keys(a->prefix_len, base, one_wave, pass, LEAST_KEYS, pl.prefix_chunk, pl.prefix_chunks);
+        else split_keys(a->prefix_len, base, one_wave(pl.prefix_nt), pass, LEAST_KEYS, pl.prefix_chunk, pl.prefix_chunks);
     }
     if ((int64_t) pl.own_tiles * pl.own_chunks > INT32_MAX || (int64_t) pl.prefix_tiles * pl.prefix_chunks > INT32_MAX)
         return fail(ctx, B200MOE_ERR_UNSUPPORTED, "too many rows");
