@@ -151,8 +151,8 @@ constexpr int CLUSTER_KEYS = 256;
 constexpr int JOIN_FEW = 32;
 // From so many rows to a key/value head the kernels with tiles of many rows run (bf16 queries); for a prefix, whose rows are the whole batch's, from more
 // than half as many.  8192 keys, Q8: 64 rows 24.1 us and 25.6 with the kernel of few rows, 128 rows 24.1 and 48.8; 16 sequences of up to
-// 4096 with 64 rows 49 and 64.  bf16, where values cost more to bring into f16: 96 rows 29.3 and 27.3, 128 rows 29.5 and 50.3.  A prefix of
-// 16000, Q8: 32 rows 28 and 27, 48 rows 29 and 48; 8192, bf16: 64 rows 29 and 29, 128 rows 30 and 53.
+// 4096 with 64 rows 49 and 64.  bf16, where values cost more to bring into f16: 96 rows 29.5 and 29.3, 128 rows 28.6 and 48.9; 16
+// sequences with 96 rows 90 and 85, with 128 91 and 103.  A prefix of 16000, Q8: 32 rows 28 and 27, 48 rows 29 and 48; 8192, bf16: 64 rows 29 and 29, 128 rows 30 and 53.
 constexpr int attn_tc_rows(int type) { return type == KV_BF16 ? 128 : 64; }
 constexpr int TC_TILE = 0;     // nt of those kernels, whose tile goes by the head_dim
 
